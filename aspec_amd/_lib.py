@@ -82,6 +82,15 @@ SIGNATURES = {
         + [_c_void_p] * 4
     ),
     "aspec_sampled_l1_bwd": (_int, [_c_void_p] * 3 + [_i64, _i64, _i64] + [_c_void_p] * 4),
+    "aspec_token_logprobs_stats_floats": (_int, []),
+    "aspec_token_logprobs_workspace_bytes": (_int, [_int, _i64, _i64, _i64, _size_p]),
+    "aspec_token_logprobs_fwd": (
+        _int, [_c_void_p, _int, _i64, _i64, _i64, _c_void_p, _i64, _f32, _i64] + [_c_void_p] * 8
+    ),
+    "aspec_token_logprobs_bwd": (
+        _int, [_c_void_p, _int, _i64, _i64, _i64, _c_void_p, _i64, _f32, _i64] + [_c_void_p] * 6
+        + [_i64, _c_void_p]
+    ),
     "aspec_pack_copy": (_int, [_c_void_p, _i64, _c_void_p]),
     "aspec_pack_row_metadata": (_int, [_c_void_p, _i64, _i64] + [_c_void_p] * 4),
     "aspec_sample_document_anchors": (
@@ -129,7 +138,7 @@ SIGNATURES = {
     "aspec_pack_work_aware_rows": (_int, [_c_void_p, _c_void_p, _i64, _i64, _i64, _i64] + [_c_void_p] * 3),
 }
 
-ABI_VERSION = 15
+ABI_VERSION = 16
 
 _lock = threading.Lock()
 _lib = None

@@ -1,0 +1,569 @@
+// Log-probabilities of given tokens, entropy and the K best alternatives of rows of logits, and
+// their gradient.
+//
+//   z = x / temperature, m = max z, S = sum exp(z - m), logp_j = z_j - m - log S, p = exp(logp)
+//   logprob = logp_t,  entropy = log S - sum exp(z - m) (z - m) / S   (two terms >= 0: no cancellation)
+//   dx_j = 1/temperature * ( -G p_j - g_H p_j (logp_j + H) + g_t [j = t] + sum_i g_i [j = top_i] ),
+//   G = g_t + sum_i g_i
+//
+// HBM-bound: the forward reads each logit once, the backward reads it once and writes the gradient
+// once. A row (or a part of a long one) lies in registers while its maximum, sums and best tokens
+// are taken.
+//
+// The K best: at least K tokens are >= the K-th largest of the threads' own maxima, and few more
+// than K of them are unless the large ones share threads. One wave finds that bound by bisection
+// over the maxima's ordered bits; the tokens at or above it go to a list in LDS, and each one's
+// place is the number of list entries above it. Order is by logit, ties by index: (ordered bits,
+// ~index) as one 64-bit number, no two alike. A list that overflows (long runs of equal logits,
+// large ones that share threads) is replaced by exactly the K best, found by bisection with counts
+// over the registers: first the K-th largest value, then the index up to which its ties belong.
+#include "vocab_rows.h"
+
+namespace aspec {
+namespace {
+
+using namespace vocab;
+
+constexpr int kStats = 4;       // per row: maximum, S, entropy, D / S
+constexpr int kList = 512;      // tokens at or above the bound that are ranked without a search
+
+struct FwdArgs {
+  const void* x;
+  int64_t rows, stride;
+  int V, parts, part_chunks, K;
+  const int64_t* ids;
+  int64_t ignore_index;
+  float inv_t;
+  float* logprobs;
+  float* entropy;
+  float* top_logprobs;
+  int64_t* top_indices;
+  float* stats;
+  float* part_sums;   // [rows][parts][3]: maximum, S, D
+  uint64_t* part_top; // [rows][parts][K], descending, 0 behind a part's last token
+  int32_t* flags;
+};
+
+struct BwdArgs {
+  const void* x;
+  int64_t rows, stride;
+  int V, parts, part_chunks, K;
+  const int64_t* ids;
+  int64_t ignore_index;
+  float inv_t;
+  const int64_t* top_indices;
+  const float* stats;
+  const float* g_logprob;
+  const float* g_entropy;
+  const float* g_top;
+  void* dx;
+  int64_t dx_stride;
+};
+
+// S and D = sum e log2 e over terms relative to m (in units of log2).
+struct Sums {
+  float m, S, D;
+  // Both relative to M >= m.
+  __device__ __forceinline__ Sums at(float M, float scale) const {
+    const float f = rebase(m, M, scale);
+    const float shift = m == kNegInf ? 0.f : (m - M) * scale;
+    // S = 0: no term, whatever the shift
+    return Sums{M, S * f, S == 0.f ? 0.f : f * fmaf(S, fmaxf(shift, -1000.f), D)};
+  }
+};
+
+// Merges the sums of the first n lanes (others hold m = -inf, S = D = 0).
+__device__ __forceinline__ Sums merge_wave(const Sums& s, float scale) {
+  Sums r = s.at(wave_allmax(s.m), scale);
+  r.S = wave_allsum(r.S);
+  r.D = wave_allsum(r.D);
+  return r;
+}
+
+struct RowResult {
+  float M, inv_t, log_s;
+  bool empty;
+  __device__ __forceinline__ float logprob(float x) const {
+    return empty ? kNegInf : (x - M) * inv_t - log_s;
+  }
+};
+
+// The row's results from its sums, written by one lane; `id` and its logit are read by the caller.
+__device__ __forceinline__ RowResult finish_row(const FwdArgs& a, int64_t row, const Sums& s, bool writer,
+                                                int64_t id, float at_id) {
+  const bool empty = s.S == 0.f;  // no finite logit: nothing has a probability
+  const float log_s = logf(s.S);
+  const RowResult r{s.m, a.inv_t, log_s, empty};
+  if (writer) {
+    const float entropy = empty ? 0.f : log_s - kLn2 * s.D / s.S;
+    a.entropy[row] = entropy;
+    *reinterpret_cast<float4*>(a.stats + row * kStats) = make_float4(s.m, s.S, entropy, empty ? 0.f : s.D / s.S);
+    if (a.ids) {
+      float lp = 0.f;
+      if (id != a.ignore_index) {
+        lp = r.logprob(at_id);
+        if (id < 0 || id >= a.V) {
+          lp = __builtin_nanf("");
+          if (a.flags) atomicOr(a.flags, 4);
+        }
+      }
+      a.logprobs[row] = lp;
+    }
+  }
+  return r;
+}
+
+template <typename E>
+__device__ __forceinline__ float logit_at(const FwdArgs& a, int64_t row, int64_t id) {
+  if (id < 0 || id >= a.V) return 0.f;
+  return E::widen(reinterpret_cast<const typename E::bits*>(a.x)[row * a.stride + id]);
+}
+
+// Block-wide count of what a thread counted; every thread gets it. `scratch` holds one word per wave.
+template <int T>
+__device__ __forceinline__ uint32_t block_count(uint32_t n, uint32_t* scratch) {
+  n = wave_allsum_u32(n);
+  if constexpr (T == 64) return n;
+  __syncthreads();  // the last count has been read
+  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = n;
+  __syncthreads();
+  uint32_t sum = 0;
+  for (int w = 0; w < T / 64; ++w) sum += scratch[w];
+  return sum;
+}
+
+template <typename E, int T, int NV, bool TOP>
+__global__ __launch_bounds__(T) void token_logprobs_kernel(FwdArgs a) {
+  constexpr int W = T / 64;
+  __shared__ float s_m[W], s_S[W], s_D[W];
+  __shared__ uint32_t s_best[TOP ? T : 1], s_count[W];
+  __shared__ uint32_t s_n, s_bound;
+  __shared__ float s_row[4];
+  __shared__ __attribute__((aligned(16))) uint64_t s_list[TOP ? kList : 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const float scale = a.inv_t * kLog2e;
+  const int64_t units = a.rows * a.parts;
+  for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const int64_t row = a.parts == 1 ? unit : unit / a.parts;
+    const int part = a.parts == 1 ? 0 : static_cast<int>(unit - row * a.parts);
+    const auto* x = reinterpret_cast<const typename E::bits*>(a.x) + row * a.stride;
+    Part<E, T, NV> p;
+    p.load(x, RowCut::at<E>(x, a.V), part, a.part_chunks);
+    int64_t id = a.ignore_index;
+    float at_id = 0.f;
+    if (a.parts == 1 && threadIdx.x == 0 && a.ids) {
+      id = a.ids[row];
+      at_id = logit_at<E>(a, row, id);
+    }
+
+    // ---- maximum and sums
+    float m = kNegInf;
+    p.each_value([&](float v) { m = fmaxf(m, v); });
+    const float wm = wave_allmax(m), base = base_of(wm);
+    float S = 0.f, D = 0.f;
+    p.each_value([&](float v) {
+      const float d = (v - base) * scale, e = fast_exp2(d);
+      S += e;
+      D = fmaf(e, fmaxf(d, -200.f), D);  // e = 0 there; -inf would make it NaN
+    });
+    S = wave_allsum(S);
+    D = wave_allsum(D);
+    if (lane == 0) {
+      s_m[wave] = wm;
+      s_S[wave] = S;
+      s_D[wave] = D;
+    }
+    if constexpr (TOP) {
+      // at most the key of the thread's largest token (the maximum skips a NaN, the highest key)
+      s_best[threadIdx.x] = order_key(m);
+      if (threadIdx.x == 0) s_n = 0;
+    }
+    __syncthreads();
+    RowResult r{0.f, 0.f, 0.f, false};
+    if (wave == 0) {
+      Sums s{kNegInf, 0.f, 0.f};
+      if (lane < W) s = Sums{s_m[lane], s_S[lane], s_D[lane]};
+      s = merge_wave(s, scale);
+      if (a.parts == 1) {
+        r = finish_row(a, row, s, lane == 0, id, at_id);
+        if constexpr (TOP) {
+          if (lane == 0) {
+            s_row[0] = r.M;
+            s_row[1] = r.log_s;
+            s_row[2] = r.empty ? 1.f : 0.f;
+          }
+        }
+      } else if (lane == 0) {
+        float* o = a.part_sums + unit * 3;
+        o[0] = s.m;
+        o[1] = s.S;
+        o[2] = s.D;
+      }
+    }
+    if constexpr (TOP) {
+      // ---- the bound: the K-th largest thread maximum, or a little below it
+      if (wave == 0) {
+        uint32_t key[W], low = 0xffffffffu, high = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          key[w] = s_best[w * 64 + lane];
+          low = min(low, key[w]);
+          high = max(high, key[w]);
+        }
+        low = wave_allmin(low);
+        high = wave_allmax_u32(high);
+        if (a.K > T) low = high = 0;  // fewer maxima than tokens wanted: every token is listed
+        const uint32_t enough = a.K + a.K / 8;
+        while (low < high) {  // count(>= low) >= K throughout
+          const uint32_t mid = low + (high - low) / 2 + ((high - low) & 1);
+          uint32_t n = 0;
+#pragma unroll
+          for (int w = 0; w < W; ++w) n += __popcll(__ballot(key[w] >= mid));
+          if (n >= static_cast<uint32_t>(a.K)) {
+            low = mid;
+            if (n <= enough) break;
+          } else {
+            high = mid - 1;
+          }
+        }
+        if (lane == 0) s_bound = low;
+      }
+      __syncthreads();
+      // ---- the list
+      const uint32_t bound = s_bound;
+      const float bound_value = key_value(bound);  // a NaN bound lists every token
+      const auto append = [&](float v, int at) {
+        const uint32_t slot = atomicAdd(&s_n, 1u);
+        if (slot < kList) s_list[slot] = ranked(order_key(v), at);
+      };
+      if (!(m < bound_value) || S != S)
+        p.each([&](float v, int at) {
+          if (!(v < bound_value)) append(v, at);
+        });
+      __syncthreads();
+      if (s_n > kList) {
+        // ---- exactly the K best: their smallest value, then the last index among its ties
+        const uint32_t K = a.K;
+        const auto count = [&](auto pred) {
+          uint32_t n = 0;
+          p.each([&](float v, int at) { n += pred(order_key(v), at) ? 1u : 0u; });
+          return block_count<T>(n, s_count);
+        };
+        uint32_t low = bound, high = 0xffffffffu;
+        if (count([&](uint32_t k, int) { return k > low; }) < K) high = low;
+        while (low < high) {
+          const uint32_t mid = low + (high - low) / 2 + ((high - low) & 1);
+          if (count([&](uint32_t k, int) { return k >= mid; }) >= K) low = mid;
+          else high = mid - 1;
+        }
+        const uint32_t above = count([&](uint32_t k, int) { return k > low; });
+        int first = 0, last = a.V - 1;
+        while (first < last) {
+          const int mid = first + (last - first) / 2;
+          if (above + count([&](uint32_t k, int at) { return k == low && at <= mid; }) >= K) last = mid;
+          else first = mid + 1;
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) s_n = 0;
+        __syncthreads();
+        p.each([&](float v, int at) {
+          const uint32_t k = order_key(v);
+          if (k > low || (k == low && at <= last)) append(v, at);
+        });
+        __syncthreads();
+      }
+      // ---- each entry's place; at least K entries, or all of a part that has fewer
+      const int n = s_n;
+      for (int i = threadIdx.x; i < n; i += T) {
+        const uint64_t mine = s_list[i];
+        int place = 0;
+        for (int j = 0; j < n; ++j) place += s_list[j] > mine ? 1 : 0;
+        if (place >= a.K) continue;
+        if (a.parts == 1) {
+          const RowResult rr{s_row[0], a.inv_t, s_row[1], s_row[2] != 0.f};
+          a.top_logprobs[row * a.K + place] = rr.logprob(ranked_value(mine));
+          a.top_indices[row * a.K + place] = ranked_index(mine);
+        } else {
+          a.part_top[unit * a.K + place] = mine;
+        }
+      }
+      if (a.parts > 1)
+        for (int i = n + threadIdx.x; i < a.K; i += T) a.part_top[unit * a.K + i] = 0;
+    }
+    __syncthreads();  // the next unit reuses the LDS
+  }
+}
+
+// Joins the parts of long rows: the sums by one wave, the ordered lists pairwise. An entry's place
+// in a pair's merged list is its own place plus the number of the other list's entries above it (a
+// binary search); entries past K are dropped.
+constexpr int kJoinThreads = 256;
+template <typename E>
+__global__ __launch_bounds__(kJoinThreads) void token_logprobs_join_kernel(FwdArgs a) {
+  __shared__ uint64_t s_a[kMaxParts * kMaxTop], s_b[kMaxParts * kMaxTop / 2];
+  __shared__ float s_row[4];
+  const int lane = threadIdx.x & 63;
+  const float scale = a.inv_t * kLog2e;
+  const int K = a.K;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    for (int i = threadIdx.x; i < a.parts * K; i += kJoinThreads) s_a[i] = a.part_top[row * a.parts * K + i];
+    if (threadIdx.x < 64) {
+      int64_t id = a.ignore_index;
+      float at_id = 0.f;
+      if (lane == 0 && a.ids) {
+        id = a.ids[row];
+        at_id = logit_at<E>(a, row, id);
+      }
+      Sums s{kNegInf, 0.f, 0.f};
+      if (lane < a.parts) {
+        const float* o = a.part_sums + (row * a.parts + lane) * 3;
+        s = Sums{o[0], o[1], o[2]};
+      }
+      s = merge_wave(s, scale);
+      const RowResult r = finish_row(a, row, s, lane == 0, id, at_id);
+      if (lane == 0) {
+        s_row[0] = r.M;
+        s_row[1] = r.log_s;
+        s_row[2] = r.empty ? 1.f : 0.f;
+      }
+    }
+    __syncthreads();
+    uint64_t *from = s_a, *to = s_b;
+    for (int lists = a.parts; lists > 1; lists = (lists + 1) / 2) {
+      for (int i = threadIdx.x; i < lists * K; i += kJoinThreads) {
+        const int list = i / K, at = i - list * K, other = list ^ 1;
+        const uint64_t mine = from[i];
+        int place = at;
+        if (other < lists) {
+          // entries of the other list before this one: larger, or equal (both 0) in the left list
+          const uint64_t* o = from + other * K;
+          int lo = 0, hi = K;
+          while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (list & 1 ? o[mid] >= mine : o[mid] > mine) lo = mid + 1;
+            else hi = mid;
+          }
+          place += lo;
+        }
+        if (place < K) to[(list / 2) * K + place] = mine;
+      }
+      __syncthreads();
+      uint64_t* t = from;
+      from = to;
+      to = t;
+    }
+    const RowResult r{s_row[0], a.inv_t, s_row[1], s_row[2] != 0.f};
+    for (int i = threadIdx.x; i < K; i += kJoinThreads) {
+      a.top_logprobs[row * K + i] = r.logprob(ranked_value(from[i]));
+      a.top_indices[row * K + i] = ranked_index(from[i]);
+    }
+    __syncthreads();
+  }
+}
+
+// Gradient: dense over a part, then the few elements that carry a token of their own, written
+// behind the dense values by the thread that wrote those.
+template <typename E, int T, int NV, bool ENTROPY>
+__global__ __launch_bounds__(T) void token_logprobs_bwd_kernel(BwdArgs a) {
+  __shared__ int s_head[T];
+  __shared__ int s_next[kMaxTop + 1], s_token[kMaxTop + 1];
+  __shared__ float s_g[kMaxTop + 1], s_value[kMaxTop + 1];
+  const float scale = a.inv_t * kLog2e;
+  const int lane = threadIdx.x & 63;
+  const int64_t units = a.rows * a.parts;
+  for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const int64_t row = a.parts == 1 ? unit : unit / a.parts;
+    const int part = a.parts == 1 ? 0 : static_cast<int>(unit - row * a.parts);
+    const auto* x = reinterpret_cast<const typename E::bits*>(a.x) + row * a.stride;
+    auto* dx = reinterpret_cast<typename E::bits*>(a.dx) + row * a.dx_stride;
+    const RowCut cut = RowCut::at<E>(dx, a.V);
+    Part<E, T, NV> p;
+    p.load(x, cut, part, a.part_chunks);
+    s_head[threadIdx.x] = -1;
+    __syncthreads();
+    // entries 0..K-1: the alternatives; entry K: the given token. Each goes to its thread's chain.
+    for (int k = threadIdx.x; k <= a.K; k += T) {
+      int64_t token = -1;
+      float g = 0.f;
+      if (k < a.K) {
+        if (a.g_top) {
+          token = a.top_indices[row * a.K + k];
+          g = a.g_top[row * a.K + k];
+        }
+      } else if (a.ids && a.g_logprob && a.ids[row] != a.ignore_index) {
+        token = a.ids[row];
+        if (token < 0 || token >= a.V) {  // the forward's check has the error; fails closed here
+          token = -1;
+          g = __builtin_nanf("");
+        } else {
+          g = a.g_logprob[row];
+        }
+      }
+      s_g[k] = g;
+      s_token[k] = static_cast<int>(token);
+      int owner = 0;
+      if (token >= 0 && token < a.V && Part<E, T, NV>::place(cut, part, a.part_chunks, static_cast<int>(token), owner) >= 0)
+        s_next[k] = atomicExch(&s_head[owner], k);
+    }
+    __syncthreads();
+    float G = 0.f;
+    for (int k = lane; k <= a.K; k += 64) G += s_g[k];
+    G = wave_allsum(G);
+    const float4 st = *reinterpret_cast<const float4*>(a.stats + row * kStats);
+    const bool empty = st.y == 0.f;  // nothing has a probability, nothing a gradient
+    const float base = base_of(st.x), inv_s = empty ? 0.f : 1.f / st.y;
+    const float gh = ENTROPY && !empty ? a.g_entropy[row] : 0.f;
+    // logp + H = ln2 (d - D / S), so dx = e (u + v d) with e = exp2(d)
+    const float v = -gh * kLn2 * inv_s * a.inv_t;
+    const float u = empty ? 0.f : (gh * kLn2 * st.w - G) * inv_s * a.inv_t;
+    const auto dense = [&](float xv) {
+      const float d = (xv - base) * scale, e = fast_exp2(d);
+      if constexpr (ENTROPY) return e * fmaf(v, fmaxf(d, -200.f), u);
+      else return e * u;
+    };
+    // the same token may be an alternative and the given one: the alternative's entry writes both
+    const int own = s_head[threadIdx.x];
+    const bool any = own >= 0;
+    if (any) {
+      for (int k = own; k >= 0; k = s_next[k]) {
+        float value = dense(E::widen(x[s_token[k]]));
+        if (!empty) {
+          value += s_g[k] * a.inv_t;
+          if (k < a.K && s_token[a.K] == s_token[k]) value += s_g[a.K] * a.inv_t;
+        }
+        s_value[k] = value;
+      }
+    }
+    p.store(dx, dense);
+    if (any) {
+      for (int k = own; k >= 0; k = s_next[k]) {
+        bool twice = false;
+        if (k == a.K)
+          for (int j = own; j >= 0; j = s_next[j]) twice |= j != k && s_token[j] == s_token[k];
+        if (!twice) dx[s_token[k]] = E::narrow(s_value[k]);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+template <typename E, int T, int NV>
+void launch_fwd(const FwdArgs& a, hipStream_t stream) {
+  const unsigned grid = grid_of(a.rows * a.parts);
+  if (a.K) token_logprobs_kernel<E, T, NV, true><<<grid, T, 0, stream>>>(a);
+  else token_logprobs_kernel<E, T, NV, false><<<grid, T, 0, stream>>>(a);
+  if (a.parts > 1) token_logprobs_join_kernel<E><<<grid_of(a.rows), kJoinThreads, 0, stream>>>(a);
+}
+
+template <typename E, int T, int NV>
+void launch_bwd(const BwdArgs& a, hipStream_t stream) {
+  const unsigned grid = grid_of(a.rows * a.parts);
+  if (a.g_entropy) token_logprobs_bwd_kernel<E, T, NV, true><<<grid, T, 0, stream>>>(a);
+  else token_logprobs_bwd_kernel<E, T, NV, false><<<grid, T, 0, stream>>>(a);
+}
+
+int check_rows(int dtype, int64_t rows, int64_t vocab, int64_t row_stride, float temperature, int64_t top_k) {
+  if (dtype != ASPEC_MASK_BF16 && dtype != ASPEC_MASK_F16 && dtype != ASPEC_MASK_F32)
+    return set_error(ASPEC_ERR_UNSUPPORTED, "token log-probabilities take bf16, fp16 or fp32 logits");
+  if (rows < 0 || vocab <= 0 || row_stride < vocab)
+    return set_error(ASPEC_ERR_INVALID, "token log-probabilities need a vocabulary and rows at least as far apart");
+  if (vocab > kMaxVocab)
+    return set_error(ASPEC_ERR_UNSUPPORTED, "token log-probabilities support at most %d logits per row",
+                     static_cast<int>(kMaxVocab));
+  if (!(temperature > 0.f) || !(1.f / temperature > 0.f) || isinf(1.f / temperature))
+    return set_error(ASPEC_ERR_INVALID, "temperature must be finite and > 0");
+  if (top_k < 0 || top_k > vocab)
+    return set_error(ASPEC_ERR_INVALID, "top_k must lie in [0, vocab]");
+  if (top_k > kMaxTop)
+    return set_error(ASPEC_ERR_UNSUPPORTED, "at most %d alternatives per row are supported", kMaxTop);
+  return ASPEC_OK;
+}
+
+}  // namespace
+}  // namespace aspec
+
+using namespace aspec;
+
+extern "C" int aspec_token_logprobs_stats_floats(void) { return kStats; }
+
+extern "C" int aspec_token_logprobs_workspace_bytes(int dtype, int64_t rows, int64_t vocab, int64_t top_k,
+                                                    size_t* bytes) {
+  if (const int e = check_rows(dtype, rows, vocab, vocab, 1.f, top_k)) return e;
+  if (!bytes) return set_error(ASPEC_ERR_INVALID, "null pointer passed to token log-probabilities");
+  const vocab::Shape s = vocab::shape_of(rows, vocab, vocab::per_chunk_of(dtype));
+  *bytes = s.parts == 1 ? 0 : static_cast<size_t>(rows) * s.parts * (top_k * 8 + 3 * 4);
+  return ASPEC_OK;
+}
+
+extern "C" int aspec_token_logprobs_fwd(const void* logits, int dtype, int64_t rows, int64_t vocab,
+                                        int64_t row_stride, const int64_t* token_ids, int64_t ignore_index,
+                                        float temperature, int64_t top_k, float* logprobs, float* entropy,
+                                        float* top_logprobs, int64_t* top_indices, float* stats,
+                                        void* workspace, int32_t* status_flags, void* stream) {
+  if (const int e = check_rows(dtype, rows, vocab, row_stride, temperature, top_k)) return e;
+  if (rows == 0) return ASPEC_OK;
+  const vocab::Shape s = vocab::shape_of(rows, vocab, vocab::per_chunk_of(dtype));
+  if (!logits || !entropy || !stats || (token_ids && !logprobs) || (top_k && (!top_logprobs || !top_indices)) ||
+      (s.parts > 1 && !workspace))
+    return set_error(ASPEC_ERR_INVALID, "null pointer passed to token log-probabilities");
+  FwdArgs a{};
+  a.x = logits;
+  a.rows = rows;
+  a.stride = row_stride;
+  a.V = static_cast<int>(vocab);
+  a.parts = static_cast<int>(s.parts);
+  a.part_chunks = static_cast<int>(s.part_chunks);
+  a.K = static_cast<int>(top_k);
+  a.ids = token_ids;
+  a.ignore_index = ignore_index;
+  a.inv_t = 1.f / temperature;
+  a.logprobs = logprobs;
+  a.entropy = entropy;
+  a.top_logprobs = top_logprobs;
+  a.top_indices = top_indices;
+  a.stats = stats;
+  a.part_top = static_cast<uint64_t*>(workspace);
+  a.part_sums = reinterpret_cast<float*>(a.part_top + rows * s.parts * top_k);
+  a.flags = status_flags;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  dispatch(dtype, s, [&](auto e, auto t, auto nv) { launch_fwd<decltype(e), t.value, nv.value>(a, st); });
+  return check_launch("token_logprobs_kernel");
+}
+
+extern "C" int aspec_token_logprobs_bwd(const void* logits, int dtype, int64_t rows, int64_t vocab,
+                                        int64_t row_stride, const int64_t* token_ids, int64_t ignore_index,
+                                        float temperature, int64_t top_k, const int64_t* top_indices,
+                                        const float* stats, const float* grad_logprobs,
+                                        const float* grad_entropy, const float* grad_top, void* grad_logits,
+                                        int64_t grad_stride, void* stream) {
+  if (const int e = check_rows(dtype, rows, vocab, row_stride, temperature, top_k)) return e;
+  if (grad_stride < vocab)
+    return set_error(ASPEC_ERR_INVALID, "token log-probabilities need a vocabulary and rows at least as far apart");
+  if (rows == 0) return ASPEC_OK;
+  if (!logits || !stats || !grad_logits || (grad_top && !top_indices) || (grad_logprobs && !token_ids))
+    return set_error(ASPEC_ERR_INVALID, "null pointer passed to the token log-probability gradient");
+  if (grad_logits == logits)
+    return set_error(ASPEC_ERR_INVALID, "the token log-probability gradient is not computed in place");
+  const vocab::Shape s = vocab::shape_of(rows, vocab, vocab::per_chunk_of(dtype));
+  BwdArgs a{};
+  a.x = logits;
+  a.rows = rows;
+  a.stride = row_stride;
+  a.V = static_cast<int>(vocab);
+  a.parts = static_cast<int>(s.parts);
+  a.part_chunks = static_cast<int>(s.part_chunks);
+  a.K = grad_top ? static_cast<int>(top_k) : 0;
+  a.ids = token_ids;
+  a.ignore_index = ignore_index;
+  a.inv_t = 1.f / temperature;
+  a.top_indices = top_indices;
+  a.stats = stats;
+  a.g_logprob = grad_logprobs;
+  a.g_entropy = grad_entropy;
+  a.g_top = grad_top;
+  a.dx = grad_logits;
+  a.dx_stride = grad_stride;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  dispatch(dtype, s, [&](auto e, auto t, auto nv) { launch_bwd<decltype(e), t.value, nv.value>(a, st); });
+  return check_launch("token_logprobs_bwd_kernel");
+}

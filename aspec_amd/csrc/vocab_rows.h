@@ -1,0 +1,308 @@
+// Rows of logits held in registers: what the token log-probability and the top-logit distillation
+// kernels share.
+//
+// A row of V logits (bf16, fp16 or fp32, any element alignment) is cut at 16-byte boundaries: the
+// interior as 16-byte chunks, dealt out to the threads of a workgroup round robin (thread t holds
+// chunks t, t + T, ...: coalesced), and up to 2 * (chunk - 1) elements before the first and after
+// the last boundary, one to a thread. So no access leaves the row and every vector access is
+// aligned, whatever the row's length and start. A row longer than T * NV chunks is cut into parts
+// of whole chunks; each part is a workgroup's.
+//
+// All exponentials are exp2((x - m) * scale) with scale = log2(e) / temperature: the difference
+// first, so nothing is rounded at the maximum itself, whatever its size.
+#pragma once
+
+#include <math.h>
+
+#include <type_traits>
+
+#include "common.h"
+
+namespace aspec {
+namespace vocab {
+
+constexpr int kMaxTop = 128;     // alternatives per row, teacher tokens per row
+constexpr int kMaxParts = 32;    // workgroups that share one row
+constexpr float kNegInf = -INFINITY;
+
+// ---- element types -------------------------------------------------------------------------------
+struct Bf16 {
+  using bits = uint16_t;
+  static constexpr int kPerChunk = 8;
+  static constexpr uint32_t kNegInfBits = 0xff80u;
+  static __device__ __forceinline__ float widen(uint16_t b) { return bf16_to_f32(b); }
+  static __device__ __forceinline__ uint16_t narrow(float f) { return f32_to_bf16_bits(f); }
+  static __device__ __forceinline__ float from_word(uint32_t w, int high) {
+    return __uint_as_float(high ? (w & 0xffff0000u) : (w << 16));
+  }
+  static __device__ __forceinline__ uint32_t to_word(float lo, float hi) { return pack_bf16x2(lo, hi); }
+};
+struct F16 {
+  using bits = uint16_t;
+  static constexpr int kPerChunk = 8;
+  static constexpr uint32_t kNegInfBits = 0xfc00u;
+  static __device__ __forceinline__ float widen(uint16_t b) {
+    return static_cast<float>(__builtin_bit_cast(_Float16, b));
+  }
+  static __device__ __forceinline__ uint16_t narrow(float f) {
+    return __builtin_bit_cast(uint16_t, static_cast<_Float16>(f));
+  }
+  static __device__ __forceinline__ float from_word(uint32_t w, int high) {
+    return widen(static_cast<uint16_t>(high ? (w >> 16) : (w & 0xffffu)));
+  }
+  static __device__ __forceinline__ uint32_t to_word(float lo, float hi) {
+    return static_cast<uint32_t>(narrow(lo)) | (static_cast<uint32_t>(narrow(hi)) << 16);
+  }
+};
+struct F32 {
+  using bits = uint32_t;
+  static constexpr int kPerChunk = 4;
+  static constexpr uint32_t kNegInfBits = 0xff800000u;
+  static __device__ __forceinline__ float widen(uint32_t b) { return __uint_as_float(b); }
+  static __device__ __forceinline__ uint32_t narrow(float f) { return __float_as_uint(f); }
+};
+
+__device__ __forceinline__ uint32_t word_of(const uint4& w, int j) {
+  return j == 0 ? w.x : j == 1 ? w.y : j == 2 ? w.z : w.w;
+}
+__device__ __forceinline__ void set_word(uint4& w, int j, uint32_t v) {
+  if (j == 0) w.x = v;
+  else if (j == 1) w.y = v;
+  else if (j == 2) w.z = v;
+  else w.w = v;
+}
+
+// Element i of a chunk (i a constant after unrolling).
+template <typename E>
+__device__ __forceinline__ float element(const uint4& w, int i) {
+  if constexpr (E::kPerChunk == 4) return __uint_as_float(word_of(w, i));
+  else return E::from_word(word_of(w, i >> 1), i & 1);
+}
+
+template <typename E>
+__device__ __forceinline__ uint4 all_neg_inf() {
+  const uint32_t v = E::kPerChunk == 4 ? E::kNegInfBits : (E::kNegInfBits | (E::kNegInfBits << 16));
+  return make_uint4(v, v, v, v);
+}
+
+// 16 bytes at any element alignment: gradient and logits rows may be aligned differently.
+template <typename E>
+__device__ __forceinline__ uint4 load16(const typename E::bits* p) {
+  return load_chunk(reinterpret_cast<const uint16_t*>(p));
+}
+template <typename E>
+__device__ __forceinline__ void store16(typename E::bits* p, const uint4& v) {
+  store_chunk(reinterpret_cast<uint16_t*>(p), v);
+}
+
+// ---- how a row is cut ----------------------------------------------------------------------------
+// `lead` elements, then `chunks` whole chunks, then the rest up to V.
+struct RowCut {
+  int lead, chunks, V;
+  template <typename E>
+  static __device__ __forceinline__ RowCut at(const void* row, int V) {
+    const int off = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(typename E::bits));
+    const int lead = min(V, (E::kPerChunk - off) % E::kPerChunk);
+    return RowCut{lead, (V - lead) / E::kPerChunk, V};
+  }
+};
+
+// One part of a row in the registers of a workgroup of T threads: chunks [c0, c1) of the row and,
+// in part 0, its edge elements (thread t < lead: element t; thread kPerChunk + t: the t-th element
+// behind the last chunk).
+template <typename E, int T, int NV>
+struct Part {
+  static constexpr int CH = E::kPerChunk;
+  uint4 w[NV];
+  float edge;     // -inf where this thread has none
+  int edge_at;    // its index in the row, or -1
+  int c0, c1;
+  RowCut cut;
+
+  __device__ __forceinline__ int chunk(int v) const { return c0 + static_cast<int>(threadIdx.x) + v * T; }
+  __device__ __forceinline__ int first(int c) const { return cut.lead + c * CH; }
+
+  __device__ __forceinline__ void load(const typename E::bits* row, const RowCut& rc, int part, int part_chunks) {
+    cut = rc;
+    c0 = part * part_chunks;
+    c1 = min(c0 + part_chunks, rc.chunks);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      w[v] = all_neg_inf<E>();
+      if (chunk(v) < c1) w[v] = load16<E>(row + first(chunk(v)));
+    }
+    edge = kNegInf;
+    edge_at = -1;
+    if (part == 0) {
+      const int t = threadIdx.x, behind = first(rc.chunks) + t - CH;
+      if (t < rc.lead) edge_at = t;
+      else if (t >= CH && behind < rc.V) edge_at = behind;
+      if (edge_at >= 0) edge = E::widen(row[edge_at]);
+    }
+  }
+
+  // f(value) of every element that the thread holds; -inf for the places it does not fill.
+  template <typename F>
+  __device__ __forceinline__ void each_value(F f) const {
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int i = 0; i < CH; ++i) f(element<E>(w[v], i));
+    f(edge);
+  }
+  // f(value, index in the row) of the elements that are there.
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+      if (chunk(v) < c1) {
+#pragma unroll
+        for (int i = 0; i < CH; ++i) f(element<E>(w[v], i), first(chunk(v)) + i);
+      }
+    if (edge_at >= 0) f(edge, edge_at);
+  }
+
+  // Where a token of the row is held: its place within the thread and, through `owner`, the thread;
+  // -1 if another part holds it.
+  static __device__ __forceinline__ int place(const RowCut& rc, int part, int part_chunks, int token, int& owner) {
+    const int in = token - rc.lead;
+    const int c = in / CH;
+    if (in >= 0 && c < rc.chunks) {
+      const int local = c - part * part_chunks;
+      if (local < 0 || local >= part_chunks) return -1;
+      owner = local % T;
+      return (local / T) * CH + in % CH;
+    }
+    if (part != 0) return -1;
+    owner = in < 0 ? token : CH + token - (rc.lead + rc.chunks * CH);
+    return NV * CH;
+  }
+  // Sets the element at a place to -inf.
+  __device__ __forceinline__ void knock_out(int at) {
+    if (at == NV * CH) edge = kNegInf;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      if (v != at / CH) continue;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t old = word_of(w[v], j);
+        uint32_t now;
+        if constexpr (CH == 4) {
+          now = at % 4 == j ? E::kNegInfBits : old;
+        } else {
+          const int i = at % 8;
+          now = i == 2 * j       ? ((old & 0xffff0000u) | E::kNegInfBits)
+                : i == 2 * j + 1 ? ((old & 0xffffu) | (E::kNegInfBits << 16))
+                                 : old;
+        }
+        set_word(w[v], j, now);
+      }
+    }
+  }
+  // Writes g(value) of every element to a row cut alike.
+  template <typename F>
+  __device__ __forceinline__ void store(typename E::bits* row, F g) const {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      if (chunk(v) >= c1) continue;
+      uint4 o;
+      if constexpr (CH == 4) {
+        o = make_uint4(E::narrow(g(element<E>(w[v], 0))), E::narrow(g(element<E>(w[v], 1))),
+                       E::narrow(g(element<E>(w[v], 2))), E::narrow(g(element<E>(w[v], 3))));
+      } else {
+        o = make_uint4(E::to_word(g(element<E>(w[v], 0)), g(element<E>(w[v], 1))),
+                       E::to_word(g(element<E>(w[v], 2)), g(element<E>(w[v], 3))),
+                       E::to_word(g(element<E>(w[v], 4)), g(element<E>(w[v], 5))),
+                       E::to_word(g(element<E>(w[v], 6)), g(element<E>(w[v], 7))));
+      }
+      store16<E>(row + first(chunk(v)), o);
+    }
+    if (edge_at >= 0) row[edge_at] = E::narrow(g(edge));
+  }
+};
+
+// A maximum to take differences from: a part without a finite logit sums exp2(-inf) = 0 terms.
+__device__ __forceinline__ float base_of(float m) { return m == kNegInf ? 0.f : m; }
+
+// The factor that takes sums relative to maximum m to ones relative to M >= m (1 where the sum has
+// no term; a NaN sum stays NaN).
+__device__ __forceinline__ float rebase(float m, float M, float scale) {
+  return m == kNegInf ? 1.f : fast_exp2((m - M) * scale);
+}
+
+// ---- order ---------------------------------------------------------------------------------------
+// Whole numbers in the order of the floats, -0 as +0 and every NaN above +inf.
+__device__ __forceinline__ uint32_t order_key(float f) {
+  uint32_t u = __float_as_uint(f);
+  if (f != f) return 0xffffffffu;
+  if (f == 0.f) u = 0u;
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
+// Larger first, then the lower index; 0 is below every token.
+__device__ __forceinline__ uint64_t ranked(uint32_t key, int index) {
+  return (static_cast<uint64_t>(key) << 32) | (0xffffffffu - static_cast<uint32_t>(index));
+}
+__device__ __forceinline__ int ranked_index(uint64_t r) {
+  return static_cast<int>(0xffffffffu - static_cast<uint32_t>(r));
+}
+__device__ __forceinline__ float ranked_value(uint64_t r) { return key_value(static_cast<uint32_t>(r >> 32)); }
+
+__device__ __forceinline__ uint32_t wave_allmax_u32(uint32_t v) {
+  return wave_allreduce_bits(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+}
+__device__ __forceinline__ uint32_t wave_allsum_u32(uint32_t v) {
+  return wave_allreduce_bits(v, [](uint32_t a, uint32_t b) { return a + b; });
+}
+__device__ __forceinline__ double wave_allsum_f64(double v) {
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
+  return v;
+}
+
+// ---- launch shapes -------------------------------------------------------------------------------
+// A shape is (threads of a workgroup, chunks a thread holds).
+struct Shape {
+  int threads, held;
+  int64_t parts, part_chunks;
+};
+constexpr int64_t kMaxVocab = int64_t{1} << 19;  // 32 parts of 4096 chunks of four fp32 logits
+
+inline int per_chunk_of(int dtype) { return dtype == ASPEC_MASK_F32 ? 4 : 8; }
+
+// Rows of up to 256 chunks take a wave each. Longer rows take workgroups of 512 threads x 8 chunks
+// where that makes two of them for each of the 256 CUs, and 256 x 4 otherwise: with few rows the
+// time is one workgroup's, and four times as many share a row.
+inline Shape shape_of(int64_t rows, int64_t V, int per_chunk) {
+  const int64_t chunks = V / per_chunk;
+  Shape s{64, 4, 1, 0};
+  if (chunks > 64 * 4) {
+    const int64_t large = (chunks + 4095) / 4096, small = (chunks + 1023) / 1024;
+    const bool many = rows * large >= 512 || small > kMaxParts;
+    s = many ? Shape{512, 8, large, 0} : Shape{256, 4, small, 0};
+  }
+  s.part_chunks = (chunks + s.parts - 1) / s.parts;
+  return s;
+}
+
+inline unsigned grid_of(int64_t units) {  // workgroups walk what is left over
+  return static_cast<unsigned>(units < (int64_t{1} << 22) ? units : (int64_t{1} << 22));
+}
+
+// f(element type, threads, chunks held) for a launch's type and shape.
+template <typename E, typename F>
+void dispatch_shape(const Shape& s, F f) {
+  if (s.threads == 64) f(E{}, std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
+  else if (s.threads == 256) f(E{}, std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
+  else f(E{}, std::integral_constant<int, 512>{}, std::integral_constant<int, 8>{});
+}
+template <typename F>
+void dispatch(int dtype, const Shape& s, F f) {
+  if (dtype == ASPEC_MASK_BF16) dispatch_shape<Bf16>(s, f);
+  else if (dtype == ASPEC_MASK_F16) dispatch_shape<F16>(s, f);
+  else dispatch_shape<F32>(s, f);
+}
+
+}  // namespace vocab
+}  // namespace aspec

@@ -1,0 +1,161 @@
+"""Log-probabilities of given tokens, entropy and the best alternatives of rows of logits, on the
+HIP kernels of csrc/token_logprobs.hip.
+
+What a scoring or verifying model answers with, and what a distillation cache keeps of a teacher
+(`aspec_amd.topk_distill` trains against `top_indices` / `top_logprobs`). One read of the logits
+forward, one read and one write backward:
+
+  logp          = log_softmax(logits / temperature)
+  logprobs      = logp[token]
+  entropy       = -sum p logp
+  top_logprobs  = the top_k largest logp, descending; ties by the lower token index
+
+No reference function matches: the reference's target engine returns hidden states, and its head
+takes the teacher's logits whole (aspec/models/dspark.py:553-612). No CPU path: the HIP library runs
+or the call raises.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import NamedTuple, Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from aspec_amd import _lib, _timing
+from aspec_amd.loss import IndexCheck
+
+_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+class TokenLogprobs(NamedTuple):
+    """Per row: fp32 `logprobs` (None without token ids), fp32 `entropy`, and, with top_k > 0, fp32
+    `top_logprobs` and int64 `top_indices` [..., top_k] (else None)."""
+
+    logprobs: Optional[torch.Tensor]
+    entropy: torch.Tensor
+    top_logprobs: Optional[torch.Tensor]
+    top_indices: Optional[torch.Tensor]
+
+
+def logit_rows(logits: torch.Tensor, what: str) -> torch.Tensor:
+    """[rows, V] of logits [..., V]: a view where the rows are evenly spaced and their elements
+    adjacent (rows padded to a longer stride among them), else a contiguous copy."""
+    if not logits.is_cuda:
+        raise ValueError(f"{what} requires CUDA logits")
+    if logits.dtype not in _DTYPES:
+        raise ValueError(f"{what} requires BF16, FP16 or FP32 logits")
+    if logits.ndim < 1 or logits.shape[-1] == 0:
+        raise ValueError(f"{what} requires logits with a vocabulary dimension")
+    vocab = logits.shape[-1]
+    rows = logits.numel() // vocab
+    flat = logits.reshape(rows, vocab)
+    if rows and (flat.stride(-1) != 1 and vocab > 1 or flat.stride(0) < vocab and rows > 1):
+        flat = flat.contiguous()  # transposed or broadcast rows
+    return flat
+
+
+def row_stride(flat: torch.Tensor) -> int:
+    return flat.stride(0) if flat.shape[0] > 1 else flat.shape[1]
+
+
+def check_temperature(temperature) -> float:
+    temperature = float(temperature)
+    if not (math.isfinite(temperature) and temperature > 0.0):
+        raise ValueError(f"temperature must be finite and > 0, got {temperature}")
+    return temperature
+
+
+def index_flags(wanted: bool, device) -> torch.Tensor | None:
+    """The zeroed flag word of a launch whose indices are to be checked. None where nothing can read
+    it: the caller wants no check, or the launch is captured into a graph, whose replays no host
+    follows."""
+    if not wanted or torch.cuda.is_current_stream_capturing():
+        return None
+    return torch.zeros(1, dtype=torch.int32, device=device)
+
+
+def settle(check: IndexCheck | None) -> None:
+    """Reads a deferred check behind the launches that it was deferred for."""
+    if check is not None and not torch.cuda.is_current_stream_capturing():
+        check.raise_if_bad()
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, top_k, temperature, ignore_index, check_ids, has_backward):
+        flat = logit_rows(logits, "token_logprobs")
+        rows, vocab = flat.shape
+        dev, lead = flat.device, logits.shape[:-1]
+        dtype = _lib.mask_dtype_code(flat)
+        lib = _lib.load()
+        with torch.cuda.device(dev):
+            size = ctypes.c_size_t()
+            _lib.check(lib.aspec_token_logprobs_workspace_bytes(dtype, rows, vocab, top_k, ctypes.byref(size)))
+            workspace = torch.empty(size.value, dtype=torch.uint8, device=dev) if size.value else None
+            entropy = torch.empty(lead, dtype=torch.float32, device=dev)
+            logprobs = torch.empty(lead, dtype=torch.float32, device=dev) if ids is not None else None
+            top = torch.empty((*lead, top_k), dtype=torch.float32, device=dev) if top_k else None
+            top_indices = torch.empty((*lead, top_k), dtype=torch.int64, device=dev) if top_k else None
+            stats = torch.empty((rows, lib.aspec_token_logprobs_stats_floats()), dtype=torch.float32, device=dev)
+            flags = index_flags(check_ids and ids is not None, dev)
+            with _timing.region("token_logprobs_fwd"):
+                _lib.call("aspec_token_logprobs_fwd", flat.data_ptr(), dtype, rows, vocab, row_stride(flat),
+                          _lib.ptr(ids), ignore_index, temperature, top_k, _lib.ptr(logprobs),
+                          entropy.data_ptr(), _lib.ptr(top), _lib.ptr(top_indices), stats.data_ptr(),
+                          _lib.ptr(workspace), _lib.ptr(flags), _lib.stream_handle(dev))
+            ctx.check = None if flags is None else IndexCheck(flags)
+        if not has_backward:
+            settle(ctx.check)
+        ctx.save_for_backward(flat, ids, top_indices, stats)
+        ctx.parameters = (top_k, temperature, ignore_index, logits.shape)
+        ctx.set_materialize_grads(False)
+        if top_indices is not None:
+            ctx.mark_non_differentiable(top_indices)
+        return logprobs, entropy, top, top_indices
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_logprobs, g_entropy, g_top, _):
+        flat, ids, top_indices, stats = ctx.saved_tensors
+        top_k, temperature, ignore_index, shape = ctx.parameters
+        rows, vocab = flat.shape
+        dev = flat.device
+        grads = [None if g is None else g.to(torch.float32).contiguous() for g in (g_logprobs, g_entropy, g_top)]
+        grad = torch.empty((rows, vocab), dtype=flat.dtype, device=dev)
+        with torch.cuda.device(dev), _timing.region("token_logprobs_bwd"):
+            _lib.call("aspec_token_logprobs_bwd", flat.data_ptr(), _lib.mask_dtype_code(flat), rows, vocab,
+                      row_stride(flat), _lib.ptr(ids), ignore_index, temperature, top_k, _lib.ptr(top_indices),
+                      stats.data_ptr(), *map(_lib.ptr, grads), grad.data_ptr(), vocab, _lib.stream_handle(dev))
+        # the forward's flag, read with this backward's kernel already queued
+        settle(ctx.check)
+        return grad.view(shape), None, None, None, None, None, None
+
+
+def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor | None = None, *, top_k: int = 0,
+                   temperature: float = 1.0, ignore_index: int = -100, check_ids: bool = True) -> TokenLogprobs:
+    """`TokenLogprobs` of logits [..., V] (bf16, fp16 or fp32, V <= 524288) in fp32, differentiable in
+    `logits` through `logprobs`, `entropy` and `top_logprobs`.
+
+    `token_ids` [...] int64: one token per row; `ignore_index` gives logprob 0 without a gradient. A
+    token outside [0, V) gives a NaN logprob (and a NaN gradient row) and raises ValueError: before
+    the call returns, or, where `logits` requires grad, from the backward, behind its kernel. Reading
+    that check waits for the GPU: with `check_ids=False` nothing waits, and the NaN is the only sign.
+    So it is in a call that is captured into a graph.
+
+    `top_k` (at most 128 and V) alternatives per row, by logit, ties by the lower index, NaN first.
+    Logits of -inf are tokens without probability (logprob -inf). A row of nothing else has logprob
+    -inf, entropy 0 and a zero gradient; one with a NaN or +inf has NaN results."""
+    temperature = check_temperature(temperature)
+    if isinstance(top_k, bool) or int(top_k) != top_k or top_k < 0:
+        raise ValueError(f"top_k must be a whole number >= 0, got {top_k}")
+    rows = logits.numel() // max(logits.shape[-1] if logits.ndim else 0, 1)
+    if token_ids is not None:
+        if token_ids.dtype != torch.int64 or token_ids.device != logits.device or (
+                token_ids.shape != logits.shape[:-1] and token_ids.shape != (rows,)):
+            raise ValueError("token_ids must be one int64 token per logit row on the logits device")
+        token_ids = token_ids.reshape(-1).contiguous()
+    return TokenLogprobs(*_TokenLogprobs.apply(logits, token_ids, int(top_k), temperature, int(ignore_index),
+                                               check_ids, torch.is_grad_enabled() and logits.requires_grad))

@@ -366,6 +366,41 @@ int aspec_sampled_l1_bwd(const void* logits, const void* teacher, const int64_t*
                          int64_t teacher_rows, int64_t rows, int64_t vocab, const float* stats,
                          const float* grad_l1, void* grad_logits, void* stream);
 
+/*
+ * Log-probabilities of given tokens, entropy and the top_k best alternatives of rows of logits. No
+ * counterpart in the reference (its target engine returns hidden states).
+ *
+ * logits [rows][row_stride >= vocab] of dtype ASPEC_MASK_BF16, ASPEC_MASK_F16 or ASPEC_MASK_F32,
+ * vocab <= 524288, any element alignment. With logp = log_softmax(logits / temperature):
+ *   logprobs[r] = logp[token_ids[r]]; 0 for ignore_index; NaN, and bit 4 of *status_flags (caller-
+ *     zeroed, may be NULL), for a token outside [0, vocab). token_ids and logprobs may be NULL.
+ *   entropy[r] = -sum p logp
+ *   top_logprobs / top_indices [rows][top_k] (top_k <= 128 and vocab; NULL with top_k 0): by logit,
+ *     descending, ties by the lower index, NaN above everything.
+ *   stats: aspec_token_logprobs_stats_floats() floats per row, for the backward.
+ * A row of -inf alone: logprobs -inf, entropy 0, no gradient. workspace: of
+ * aspec_token_logprobs_workspace_bytes (0 for most shapes; uninitialised; free once the call's
+ * kernels are done).
+ *
+ * aspec_token_logprobs_bwd writes the gradient of
+ * sum (grad_logprobs logprobs + grad_entropy entropy + grad_top top_logprobs) (each may be NULL) in
+ * the logits' dtype to grad_logits [rows][grad_stride], which is not the logits' buffer.
+ */
+int aspec_token_logprobs_stats_floats(void);
+int aspec_token_logprobs_workspace_bytes(int dtype, int64_t rows, int64_t vocab, int64_t top_k,
+                                         size_t* bytes);
+int aspec_token_logprobs_fwd(const void* logits, int dtype, int64_t rows, int64_t vocab,
+                             int64_t row_stride, const int64_t* token_ids, int64_t ignore_index,
+                             float temperature, int64_t top_k, float* logprobs, float* entropy,
+                             float* top_logprobs, int64_t* top_indices, float* stats, void* workspace,
+                             int32_t* status_flags, void* stream);
+int aspec_token_logprobs_bwd(const void* logits, int dtype, int64_t rows, int64_t vocab,
+                             int64_t row_stride, const int64_t* token_ids, int64_t ignore_index,
+                             float temperature, int64_t top_k, const int64_t* top_indices,
+                             const float* stats, const float* grad_logprobs,
+                             const float* grad_entropy, const float* grad_top, void* grad_logits,
+                             int64_t grad_stride, void* stream);
+
 /* ---------------------------------------------------------------------------------------------
  * Row-level operations around the attention and loss: packing, anchors, output blocks, targets.
  * ------------------------------------------------------------------------------------------- */
