@@ -64,6 +64,7 @@ from aspec_amd.thd_attention import thd_fa4_attention  # noqa: F401
 from aspec_amd.thd_sparse_metadata import build_thd_sparse_pair  # noqa: F401
 from aspec_amd.tiled_l1 import tiled_l1_from_logits  # noqa: F401
 from aspec_amd.token_logprobs import TokenLogprobs, token_logprobs  # noqa: F401
+from aspec_amd.topk_distill import topk_distill_from_logits, topk_distill_fused_grad  # noqa: F401
 
 __all__ = [
     "AcceptRatePredictor",
@@ -108,4 +109,6 @@ __all__ = [
     "tiled_l1_from_logits",
     "TokenLogprobs",
     "token_logprobs",
+    "topk_distill_from_logits",
+    "topk_distill_fused_grad",
 ]

@@ -91,6 +91,20 @@ SIGNATURES = {
         _int, [_c_void_p, _int, _i64, _i64, _i64, _c_void_p, _i64, _f32, _i64] + [_c_void_p] * 6
         + [_i64, _c_void_p]
     ),
+    "aspec_topk_distill_stats_floats": (_int, []),
+    "aspec_topk_distill_workspace_bytes": (_int, [_int, _i64, _i64, _size_p]),
+    "aspec_topk_distill_fwd": (
+        _int, [_c_void_p, _int, _i64, _i64, _i64, _c_void_p, _i64, _c_void_p, _int, _c_void_p, _i64, _c_void_p,
+               _i64, _int, _f32] + [_c_void_p] * 8
+    ),
+    "aspec_topk_distill_bwd": (
+        _int, [_c_void_p, _int, _i64, _i64, _i64, _c_void_p, _i64, _c_void_p, _int, _c_void_p, _i64, _c_void_p,
+               _i64, _f32] + [_c_void_p] * 4 + [_i64, _c_void_p]
+    ),
+    "aspec_topk_distill_fused_fwd_bwd": (
+        _int, [_c_void_p, _int, _i64, _i64, _i64, _c_void_p, _i64, _c_void_p, _int, _c_void_p, _i64, _c_void_p,
+               _i64, _int, _f32] + [_c_void_p] * 9 + [_i64, _c_void_p, _c_void_p]
+    ),
     "aspec_pack_copy": (_int, [_c_void_p, _i64, _c_void_p]),
     "aspec_pack_row_metadata": (_int, [_c_void_p, _i64, _i64] + [_c_void_p] * 4),
     "aspec_sample_document_anchors": (

@@ -133,7 +133,7 @@ __device__ __forceinline__ uint32_t block_count(uint32_t n, uint32_t* scratch) {
 }
 
 template <typename E, int T, int NV, bool TOP>
-__global__ __launch_bounds__(T) void token_logprobs_kernel(FwdArgs a) {
+__global__ __launch_bounds__(T, min_waves(T)) void token_logprobs_kernel(FwdArgs a) {
   constexpr int W = T / 64;
   __shared__ float s_m[W], s_S[W], s_D[W];
   __shared__ uint32_t s_best[TOP ? T : 1], s_count[W];
@@ -142,155 +142,156 @@ __global__ __launch_bounds__(T) void token_logprobs_kernel(FwdArgs a) {
   __shared__ __attribute__((aligned(16))) uint64_t s_list[TOP ? kList : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float scale = a.inv_t * kLog2e;
-  const int64_t units = a.rows * a.parts;
-  for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
-    const int64_t row = a.parts == 1 ? unit : unit / a.parts;
-    const int part = a.parts == 1 ? 0 : static_cast<int>(unit - row * a.parts);
-    const auto* x = reinterpret_cast<const typename E::bits*>(a.x) + row * a.stride;
-    Part<E, T, NV> p;
-    p.load(x, RowCut::at<E>(x, a.V), part, a.part_chunks);
-    int64_t id = a.ignore_index;
-    float at_id = 0.f;
-    if (a.parts == 1 && threadIdx.x == 0 && a.ids) {
-      id = a.ids[row];
-      at_id = logit_at<E>(a, row, id);
-    }
+  const int64_t unit = unit_of_block();
+  if (unit >= a.rows * a.parts) return;
+  const int64_t row = a.parts == 1 ? unit : unit / a.parts;
+  const int part = a.parts == 1 ? 0 : static_cast<int>(unit - row * a.parts);
+  const auto* x = reinterpret_cast<const typename E::bits*>(a.x) + row * a.stride;
+  Part<E, T, NV> p;
+  p.load(x, RowCut::at<E>(x, a.V), part, a.part_chunks);
+  int64_t id = a.ignore_index;
+  float at_id = 0.f;
+  if (a.parts == 1 && threadIdx.x == 0 && a.ids) {
+    id = a.ids[row];
+    at_id = logit_at<E>(a, row, id);
+  }
 
-    // ---- maximum and sums
-    float m = kNegInf;
-    p.each_value([&](float v) { m = fmaxf(m, v); });
-    const float wm = wave_allmax(m), base = base_of(wm);
-    float S = 0.f, D = 0.f;
-    p.each_value([&](float v) {
-      const float d = (v - base) * scale, e = fast_exp2(d);
-      S += e;
-      D = fmaf(e, fmaxf(d, -200.f), D);  // e = 0 there; -inf would make it NaN
-    });
-    S = wave_allsum(S);
-    D = wave_allsum(D);
-    if (lane == 0) {
-      s_m[wave] = wm;
-      s_S[wave] = S;
-      s_D[wave] = D;
+  // ---- maximum and sums
+  float m = kNegInf;
+  p.each_value([&](float v) { m = fmaxf(m, v); });
+  const float wm = wave_allmax(m), base = base_of(wm);
+  p.forget();
+  float S = 0.f, D = 0.f;
+  p.each_value([&](float v) {
+    const float d = (v - base) * scale, e = fast_exp2(d);
+    S += e;
+    D = fmaf(e, fmaxf(d, -200.f), D);  // e = 0 there; -inf would make it NaN
+  });
+  p.forget();
+  S = wave_allsum(S);
+  D = wave_allsum(D);
+  if (lane == 0) {
+    s_m[wave] = wm;
+    s_S[wave] = S;
+    s_D[wave] = D;
+  }
+  if constexpr (TOP) {
+    // at most the key of the thread's largest token (the maximum skips a NaN, the highest key)
+    s_best[threadIdx.x] = order_key(m);
+    if (threadIdx.x == 0) s_n = 0;
+  }
+  __syncthreads();
+  RowResult r{0.f, 0.f, 0.f, false};
+  if (wave == 0) {
+    Sums s{kNegInf, 0.f, 0.f};
+    if (lane < W) s = Sums{s_m[lane], s_S[lane], s_D[lane]};
+    s = merge_wave(s, scale);
+    if (a.parts == 1) {
+      r = finish_row(a, row, s, lane == 0, id, at_id);
+      if constexpr (TOP) {
+        if (lane == 0) {
+          s_row[0] = r.M;
+          s_row[1] = r.log_s;
+          s_row[2] = r.empty ? 1.f : 0.f;
+        }
+      }
+    } else if (lane == 0) {
+      float* o = a.part_sums + unit * 3;
+      o[0] = s.m;
+      o[1] = s.S;
+      o[2] = s.D;
     }
-    if constexpr (TOP) {
-      // at most the key of the thread's largest token (the maximum skips a NaN, the highest key)
-      s_best[threadIdx.x] = order_key(m);
-      if (threadIdx.x == 0) s_n = 0;
+  }
+  if constexpr (TOP) {
+    // ---- the bound: the K-th largest thread maximum, or a little below it
+    if (wave == 0) {
+      uint32_t key[W], low = 0xffffffffu, high = 0;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        key[w] = s_best[w * 64 + lane];
+        low = min(low, key[w]);
+        high = max(high, key[w]);
+      }
+      low = wave_allmin(low);
+      high = wave_allmax_u32(high);
+      if (a.K > T) low = high = 0;  // fewer maxima than tokens wanted: every token is listed
+      const uint32_t enough = a.K + a.K / 8;
+      while (low < high) {  // count(>= low) >= K throughout
+        const uint32_t mid = low + (high - low) / 2 + ((high - low) & 1);
+        uint32_t n = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) n += __popcll(__ballot(key[w] >= mid));
+        if (n >= static_cast<uint32_t>(a.K)) {
+          low = mid;
+          if (n <= enough) break;
+        } else {
+          high = mid - 1;
+        }
+      }
+      if (lane == 0) s_bound = low;
     }
     __syncthreads();
-    RowResult r{0.f, 0.f, 0.f, false};
-    if (wave == 0) {
-      Sums s{kNegInf, 0.f, 0.f};
-      if (lane < W) s = Sums{s_m[lane], s_S[lane], s_D[lane]};
-      s = merge_wave(s, scale);
-      if (a.parts == 1) {
-        r = finish_row(a, row, s, lane == 0, id, at_id);
-        if constexpr (TOP) {
-          if (lane == 0) {
-            s_row[0] = r.M;
-            s_row[1] = r.log_s;
-            s_row[2] = r.empty ? 1.f : 0.f;
-          }
-        }
-      } else if (lane == 0) {
-        float* o = a.part_sums + unit * 3;
-        o[0] = s.m;
-        o[1] = s.S;
-        o[2] = s.D;
-      }
-    }
-    if constexpr (TOP) {
-      // ---- the bound: the K-th largest thread maximum, or a little below it
-      if (wave == 0) {
-        uint32_t key[W], low = 0xffffffffu, high = 0;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-          key[w] = s_best[w * 64 + lane];
-          low = min(low, key[w]);
-          high = max(high, key[w]);
-        }
-        low = wave_allmin(low);
-        high = wave_allmax_u32(high);
-        if (a.K > T) low = high = 0;  // fewer maxima than tokens wanted: every token is listed
-        const uint32_t enough = a.K + a.K / 8;
-        while (low < high) {  // count(>= low) >= K throughout
-          const uint32_t mid = low + (high - low) / 2 + ((high - low) & 1);
-          uint32_t n = 0;
-#pragma unroll
-          for (int w = 0; w < W; ++w) n += __popcll(__ballot(key[w] >= mid));
-          if (n >= static_cast<uint32_t>(a.K)) {
-            low = mid;
-            if (n <= enough) break;
-          } else {
-            high = mid - 1;
-          }
-        }
-        if (lane == 0) s_bound = low;
-      }
-      __syncthreads();
-      // ---- the list
-      const uint32_t bound = s_bound;
-      const float bound_value = key_value(bound);  // a NaN bound lists every token
-      const auto append = [&](float v, int at) {
-        const uint32_t slot = atomicAdd(&s_n, 1u);
-        if (slot < kList) s_list[slot] = ranked(order_key(v), at);
+    // ---- the list
+    const uint32_t bound = s_bound;
+    const float bound_value = key_value(bound);  // a NaN bound lists every token
+    const auto append = [&](float v, int at) {
+      const uint32_t slot = atomicAdd(&s_n, 1u);
+      if (slot < kList) s_list[slot] = ranked(order_key(v), at);
+    };
+    if (!(m < bound_value) || S != S)
+      p.each([&](float v, int at) {
+        if (!(v < bound_value)) append(v, at);
+      });
+    __syncthreads();
+    if (s_n > kList) {
+      // ---- exactly the K best: their smallest value, then the last index among its ties
+      const uint32_t K = a.K;
+      const auto count = [&](auto pred) {
+        uint32_t n = 0;
+        p.forget();
+        p.each([&](float v, int at) { n += pred(order_key(v), at) ? 1u : 0u; });
+        return block_count<T>(n, s_count);
       };
-      if (!(m < bound_value) || S != S)
-        p.each([&](float v, int at) {
-          if (!(v < bound_value)) append(v, at);
-        });
+      uint32_t low = bound, high = 0xffffffffu;
+      if (count([&](uint32_t k, int) { return k > low; }) < K) high = low;
+      while (low < high) {
+        const uint32_t mid = low + (high - low) / 2 + ((high - low) & 1);
+        if (count([&](uint32_t k, int) { return k >= mid; }) >= K) low = mid;
+        else high = mid - 1;
+      }
+      const uint32_t above = count([&](uint32_t k, int) { return k > low; });
+      int first = 0, last = a.V - 1;
+      while (first < last) {
+        const int mid = first + (last - first) / 2;
+        if (above + count([&](uint32_t k, int at) { return k == low && at <= mid; }) >= K) last = mid;
+        else first = mid + 1;
+      }
       __syncthreads();
-      if (s_n > kList) {
-        // ---- exactly the K best: their smallest value, then the last index among its ties
-        const uint32_t K = a.K;
-        const auto count = [&](auto pred) {
-          uint32_t n = 0;
-          p.each([&](float v, int at) { n += pred(order_key(v), at) ? 1u : 0u; });
-          return block_count<T>(n, s_count);
-        };
-        uint32_t low = bound, high = 0xffffffffu;
-        if (count([&](uint32_t k, int) { return k > low; }) < K) high = low;
-        while (low < high) {
-          const uint32_t mid = low + (high - low) / 2 + ((high - low) & 1);
-          if (count([&](uint32_t k, int) { return k >= mid; }) >= K) low = mid;
-          else high = mid - 1;
-        }
-        const uint32_t above = count([&](uint32_t k, int) { return k > low; });
-        int first = 0, last = a.V - 1;
-        while (first < last) {
-          const int mid = first + (last - first) / 2;
-          if (above + count([&](uint32_t k, int at) { return k == low && at <= mid; }) >= K) last = mid;
-          else first = mid + 1;
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) s_n = 0;
-        __syncthreads();
-        p.each([&](float v, int at) {
-          const uint32_t k = order_key(v);
-          if (k > low || (k == low && at <= last)) append(v, at);
-        });
-        __syncthreads();
-      }
-      // ---- each entry's place; at least K entries, or all of a part that has fewer
-      const int n = s_n;
-      for (int i = threadIdx.x; i < n; i += T) {
-        const uint64_t mine = s_list[i];
-        int place = 0;
-        for (int j = 0; j < n; ++j) place += s_list[j] > mine ? 1 : 0;
-        if (place >= a.K) continue;
-        if (a.parts == 1) {
-          const RowResult rr{s_row[0], a.inv_t, s_row[1], s_row[2] != 0.f};
-          a.top_logprobs[row * a.K + place] = rr.logprob(ranked_value(mine));
-          a.top_indices[row * a.K + place] = ranked_index(mine);
-        } else {
-          a.part_top[unit * a.K + place] = mine;
-        }
-      }
-      if (a.parts > 1)
-        for (int i = n + threadIdx.x; i < a.K; i += T) a.part_top[unit * a.K + i] = 0;
+      if (threadIdx.x == 0) s_n = 0;
+      __syncthreads();
+      p.each([&](float v, int at) {
+        const uint32_t k = order_key(v);
+        if (k > low || (k == low && at <= last)) append(v, at);
+      });
+      __syncthreads();
     }
-    __syncthreads();  // the next unit reuses the LDS
+    // ---- each entry's place; at least K entries, or all of a part that has fewer
+    const int n = s_n;
+    for (int i = threadIdx.x; i < n; i += T) {
+      const uint64_t mine = s_list[i];
+      int place = 0;
+      for (int j = 0; j < n; ++j) place += s_list[j] > mine ? 1 : 0;
+      if (place >= a.K) continue;
+      if (a.parts == 1) {
+        const RowResult rr{s_row[0], a.inv_t, s_row[1], s_row[2] != 0.f};
+        a.top_logprobs[row * a.K + place] = rr.logprob(ranked_value(mine));
+        a.top_indices[row * a.K + place] = ranked_index(mine);
+      } else {
+        a.part_top[unit * a.K + place] = mine;
+      }
+    }
+    if (a.parts > 1)
+      for (int i = n + threadIdx.x; i < a.K; i += T) a.part_top[unit * a.K + i] = 0;
   }
 }
 
@@ -305,151 +306,148 @@ __global__ __launch_bounds__(kJoinThreads) void token_logprobs_join_kernel(FwdAr
   const int lane = threadIdx.x & 63;
   const float scale = a.inv_t * kLog2e;
   const int K = a.K;
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    for (int i = threadIdx.x; i < a.parts * K; i += kJoinThreads) s_a[i] = a.part_top[row * a.parts * K + i];
-    if (threadIdx.x < 64) {
-      int64_t id = a.ignore_index;
-      float at_id = 0.f;
-      if (lane == 0 && a.ids) {
-        id = a.ids[row];
-        at_id = logit_at<E>(a, row, id);
-      }
-      Sums s{kNegInf, 0.f, 0.f};
-      if (lane < a.parts) {
-        const float* o = a.part_sums + (row * a.parts + lane) * 3;
-        s = Sums{o[0], o[1], o[2]};
-      }
-      s = merge_wave(s, scale);
-      const RowResult r = finish_row(a, row, s, lane == 0, id, at_id);
-      if (lane == 0) {
-        s_row[0] = r.M;
-        s_row[1] = r.log_s;
-        s_row[2] = r.empty ? 1.f : 0.f;
-      }
+  const int64_t row = unit_of_block();
+  if (row >= a.rows) return;
+  for (int i = threadIdx.x; i < a.parts * K; i += kJoinThreads) s_a[i] = a.part_top[row * a.parts * K + i];
+  if (threadIdx.x < 64) {
+    int64_t id = a.ignore_index;
+    float at_id = 0.f;
+    if (lane == 0 && a.ids) {
+      id = a.ids[row];
+      at_id = logit_at<E>(a, row, id);
     }
-    __syncthreads();
-    uint64_t *from = s_a, *to = s_b;
-    for (int lists = a.parts; lists > 1; lists = (lists + 1) / 2) {
-      for (int i = threadIdx.x; i < lists * K; i += kJoinThreads) {
-        const int list = i / K, at = i - list * K, other = list ^ 1;
-        const uint64_t mine = from[i];
-        int place = at;
-        if (other < lists) {
-          // entries of the other list before this one: larger, or equal (both 0) in the left list
-          const uint64_t* o = from + other * K;
-          int lo = 0, hi = K;
-          while (lo < hi) {
-            const int mid = (lo + hi) / 2;
-            if (list & 1 ? o[mid] >= mine : o[mid] > mine) lo = mid + 1;
-            else hi = mid;
-          }
-          place += lo;
+    Sums s{kNegInf, 0.f, 0.f};
+    if (lane < a.parts) {
+      const float* o = a.part_sums + (row * a.parts + lane) * 3;
+      s = Sums{o[0], o[1], o[2]};
+    }
+    s = merge_wave(s, scale);
+    const RowResult r = finish_row(a, row, s, lane == 0, id, at_id);
+    if (lane == 0) {
+      s_row[0] = r.M;
+      s_row[1] = r.log_s;
+      s_row[2] = r.empty ? 1.f : 0.f;
+    }
+  }
+  __syncthreads();
+  uint64_t *from = s_a, *to = s_b;
+  for (int lists = a.parts; lists > 1; lists = (lists + 1) / 2) {
+    for (int i = threadIdx.x; i < lists * K; i += kJoinThreads) {
+      const int list = i / K, at = i - list * K, other = list ^ 1;
+      const uint64_t mine = from[i];
+      int place = at;
+      if (other < lists) {
+        // entries of the other list before this one: larger, or equal (both 0) in the left list
+        const uint64_t* o = from + other * K;
+        int lo = 0, hi = K;
+        while (lo < hi) {
+          const int mid = (lo + hi) / 2;
+          if (list & 1 ? o[mid] >= mine : o[mid] > mine) lo = mid + 1;
+          else hi = mid;
         }
-        if (place < K) to[(list / 2) * K + place] = mine;
+        place += lo;
       }
-      __syncthreads();
-      uint64_t* t = from;
-      from = to;
-      to = t;
-    }
-    const RowResult r{s_row[0], a.inv_t, s_row[1], s_row[2] != 0.f};
-    for (int i = threadIdx.x; i < K; i += kJoinThreads) {
-      a.top_logprobs[row * K + i] = r.logprob(ranked_value(from[i]));
-      a.top_indices[row * K + i] = ranked_index(from[i]);
+      if (place < K) to[(list / 2) * K + place] = mine;
     }
     __syncthreads();
+    uint64_t* t = from;
+    from = to;
+    to = t;
+  }
+  const RowResult r{s_row[0], a.inv_t, s_row[1], s_row[2] != 0.f};
+  for (int i = threadIdx.x; i < K; i += kJoinThreads) {
+    a.top_logprobs[row * K + i] = r.logprob(ranked_value(from[i]));
+    a.top_indices[row * K + i] = ranked_index(from[i]);
   }
 }
 
 // Gradient: dense over a part, then the few elements that carry a token of their own, written
 // behind the dense values by the thread that wrote those.
 template <typename E, int T, int NV, bool ENTROPY>
-__global__ __launch_bounds__(T) void token_logprobs_bwd_kernel(BwdArgs a) {
+__global__ __launch_bounds__(T, min_waves(T)) void token_logprobs_bwd_kernel(BwdArgs a) {
   __shared__ int s_head[T];
   __shared__ int s_next[kMaxTop + 1], s_token[kMaxTop + 1];
   __shared__ float s_g[kMaxTop + 1], s_value[kMaxTop + 1];
   const float scale = a.inv_t * kLog2e;
   const int lane = threadIdx.x & 63;
-  const int64_t units = a.rows * a.parts;
-  for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
-    const int64_t row = a.parts == 1 ? unit : unit / a.parts;
-    const int part = a.parts == 1 ? 0 : static_cast<int>(unit - row * a.parts);
-    const auto* x = reinterpret_cast<const typename E::bits*>(a.x) + row * a.stride;
-    auto* dx = reinterpret_cast<typename E::bits*>(a.dx) + row * a.dx_stride;
-    const RowCut cut = RowCut::at<E>(dx, a.V);
-    Part<E, T, NV> p;
-    p.load(x, cut, part, a.part_chunks);
-    s_head[threadIdx.x] = -1;
-    __syncthreads();
-    // entries 0..K-1: the alternatives; entry K: the given token. Each goes to its thread's chain.
-    for (int k = threadIdx.x; k <= a.K; k += T) {
-      int64_t token = -1;
-      float g = 0.f;
-      if (k < a.K) {
-        if (a.g_top) {
-          token = a.top_indices[row * a.K + k];
-          g = a.g_top[row * a.K + k];
-        }
-      } else if (a.ids && a.g_logprob && a.ids[row] != a.ignore_index) {
-        token = a.ids[row];
-        if (token < 0 || token >= a.V) {  // the forward's check has the error; fails closed here
-          token = -1;
-          g = __builtin_nanf("");
-        } else {
-          g = a.g_logprob[row];
-        }
+  const int64_t unit = unit_of_block();
+  if (unit >= a.rows * a.parts) return;
+  const int64_t row = a.parts == 1 ? unit : unit / a.parts;
+  const int part = a.parts == 1 ? 0 : static_cast<int>(unit - row * a.parts);
+  const auto* x = reinterpret_cast<const typename E::bits*>(a.x) + row * a.stride;
+  auto* dx = reinterpret_cast<typename E::bits*>(a.dx) + row * a.dx_stride;
+  const RowCut cut = RowCut::at<E>(dx, a.V);
+  Part<E, T, NV> p;
+  p.load(x, cut, part, a.part_chunks);
+  s_head[threadIdx.x] = -1;
+  __syncthreads();
+  // entries 0..K-1: the alternatives; entry K: the given token. Each goes to its thread's chain.
+  for (int k = threadIdx.x; k <= a.K; k += T) {
+    int64_t token = -1;
+    float g = 0.f;
+    if (k < a.K) {
+      if (a.g_top) {
+        token = a.top_indices[row * a.K + k];
+        g = a.g_top[row * a.K + k];
       }
-      s_g[k] = g;
-      s_token[k] = static_cast<int>(token);
-      int owner = 0;
-      if (token >= 0 && token < a.V && Part<E, T, NV>::place(cut, part, a.part_chunks, static_cast<int>(token), owner) >= 0)
-        s_next[k] = atomicExch(&s_head[owner], k);
-    }
-    __syncthreads();
-    float G = 0.f;
-    for (int k = lane; k <= a.K; k += 64) G += s_g[k];
-    G = wave_allsum(G);
-    const float4 st = *reinterpret_cast<const float4*>(a.stats + row * kStats);
-    const bool empty = st.y == 0.f;  // nothing has a probability, nothing a gradient
-    const float base = base_of(st.x), inv_s = empty ? 0.f : 1.f / st.y;
-    const float gh = ENTROPY && !empty ? a.g_entropy[row] : 0.f;
-    // logp + H = ln2 (d - D / S), so dx = e (u + v d) with e = exp2(d)
-    const float v = -gh * kLn2 * inv_s * a.inv_t;
-    const float u = empty ? 0.f : (gh * kLn2 * st.w - G) * inv_s * a.inv_t;
-    const auto dense = [&](float xv) {
-      const float d = (xv - base) * scale, e = fast_exp2(d);
-      if constexpr (ENTROPY) return e * fmaf(v, fmaxf(d, -200.f), u);
-      else return e * u;
-    };
-    // the same token may be an alternative and the given one: the alternative's entry writes both
-    const int own = s_head[threadIdx.x];
-    const bool any = own >= 0;
-    if (any) {
-      for (int k = own; k >= 0; k = s_next[k]) {
-        float value = dense(E::widen(x[s_token[k]]));
-        if (!empty) {
-          value += s_g[k] * a.inv_t;
-          if (k < a.K && s_token[a.K] == s_token[k]) value += s_g[a.K] * a.inv_t;
-        }
-        s_value[k] = value;
+    } else if (a.ids && a.g_logprob && a.ids[row] != a.ignore_index) {
+      token = a.ids[row];
+      if (token < 0 || token >= a.V) {  // the forward's check has the error; fails closed here
+        token = -1;
+        g = __builtin_nanf("");
+      } else {
+        g = a.g_logprob[row];
       }
     }
-    p.store(dx, dense);
-    if (any) {
-      for (int k = own; k >= 0; k = s_next[k]) {
-        bool twice = false;
-        if (k == a.K)
-          for (int j = own; j >= 0; j = s_next[j]) twice |= j != k && s_token[j] == s_token[k];
-        if (!twice) dx[s_token[k]] = E::narrow(s_value[k]);
+    s_g[k] = g;
+    s_token[k] = static_cast<int>(token);
+    int owner = 0;
+    if (token >= 0 && token < a.V && Part<E, T, NV>::place(cut, part, a.part_chunks, static_cast<int>(token), owner) >= 0)
+      s_next[k] = atomicExch(&s_head[owner], k);
+  }
+  __syncthreads();
+  float G = 0.f;
+  for (int k = lane; k <= a.K; k += 64) G += s_g[k];
+  G = wave_allsum(G);
+  const float4 st = *reinterpret_cast<const float4*>(a.stats + row * kStats);
+  const bool empty = st.y == 0.f;  // nothing has a probability, nothing a gradient
+  const float base = base_of(st.x), inv_s = empty ? 0.f : 1.f / st.y;
+  const float gh = ENTROPY && !empty ? a.g_entropy[row] : 0.f;
+  // logp + H = ln2 (d - D / S), so dx = e (u + v d) with e = exp2(d)
+  const float v = -gh * kLn2 * inv_s * a.inv_t;
+  const float u = empty ? 0.f : (gh * kLn2 * st.w - G) * inv_s * a.inv_t;
+  const auto dense = [&](float xv) {
+    const float d = (xv - base) * scale, e = fast_exp2(d);
+    if constexpr (ENTROPY) return e * fmaf(v, fmaxf(d, -200.f), u);
+    else return e * u;
+  };
+  // the same token may be an alternative and the given one: the alternative's entry writes both
+  const int own = s_head[threadIdx.x];
+  const bool any = own >= 0;
+  if (any) {
+    for (int k = own; k >= 0; k = s_next[k]) {
+      float value = dense(E::widen(x[s_token[k]]));
+      if (!empty) {
+        value += s_g[k] * a.inv_t;
+        if (k < a.K && s_token[a.K] == s_token[k]) value += s_g[a.K] * a.inv_t;
       }
+      s_value[k] = value;
     }
-    __syncthreads();
+  }
+  p.store(dx, dense);
+  if (any) {
+    for (int k = own; k >= 0; k = s_next[k]) {
+      bool twice = false;
+      if (k == a.K)
+        for (int j = own; j >= 0; j = s_next[j]) twice |= j != k && s_token[j] == s_token[k];
+      if (!twice) dx[s_token[k]] = E::narrow(s_value[k]);
+    }
   }
 }
 
 template <typename E, int T, int NV>
 void launch_fwd(const FwdArgs& a, hipStream_t stream) {
-  const unsigned grid = grid_of(a.rows * a.parts);
+  const dim3 grid = grid_of(a.rows * a.parts);
   if (a.K) token_logprobs_kernel<E, T, NV, true><<<grid, T, 0, stream>>>(a);
   else token_logprobs_kernel<E, T, NV, false><<<grid, T, 0, stream>>>(a);
   if (a.parts > 1) token_logprobs_join_kernel<E><<<grid_of(a.rows), kJoinThreads, 0, stream>>>(a);
@@ -457,7 +455,7 @@ void launch_fwd(const FwdArgs& a, hipStream_t stream) {
 
 template <typename E, int T, int NV>
 void launch_bwd(const BwdArgs& a, hipStream_t stream) {
-  const unsigned grid = grid_of(a.rows * a.parts);
+  const dim3 grid = grid_of(a.rows * a.parts);
   if (a.g_entropy) token_logprobs_bwd_kernel<E, T, NV, true><<<grid, T, 0, stream>>>(a);
   else token_logprobs_bwd_kernel<E, T, NV, false><<<grid, T, 0, stream>>>(a);
 }

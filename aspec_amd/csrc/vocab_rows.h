@@ -85,14 +85,18 @@ __device__ __forceinline__ uint4 all_neg_inf() {
   return make_uint4(v, v, v, v);
 }
 
-// 16 bytes at any element alignment: gradient and logits rows may be aligned differently.
+// 16 bytes of a row from element `at` on, at any element alignment: gradient and logits rows may be
+// aligned differently. The byte offset has 32 bits (rows have at most 2 MB), so that the row's
+// address stays in scalar registers.
 template <typename E>
-__device__ __forceinline__ uint4 load16(const typename E::bits* p) {
-  return load_chunk(reinterpret_cast<const uint16_t*>(p));
+__device__ __forceinline__ uint4 load16(const typename E::bits* row, int at) {
+  const uint32_t off = static_cast<uint32_t>(at) * static_cast<uint32_t>(sizeof(typename E::bits));
+  return load_chunk(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(row) + off));
 }
 template <typename E>
-__device__ __forceinline__ void store16(typename E::bits* p, const uint4& v) {
-  store_chunk(reinterpret_cast<uint16_t*>(p), v);
+__device__ __forceinline__ void store16(typename E::bits* row, int at, const uint4& v) {
+  const uint32_t off = static_cast<uint32_t>(at) * static_cast<uint32_t>(sizeof(typename E::bits));
+  store_chunk(reinterpret_cast<uint16_t*>(reinterpret_cast<char*>(row) + off), v);
 }
 
 // ---- how a row is cut ----------------------------------------------------------------------------
@@ -116,29 +120,35 @@ struct Part {
   uint4 w[NV];
   float edge;     // -inf where this thread has none
   int edge_at;    // its index in the row, or -1
-  int c0, c1;
-  RowCut cut;
-
-  __device__ __forceinline__ int chunk(int v) const { return c0 + static_cast<int>(threadIdx.x) + v * T; }
-  __device__ __forceinline__ int first(int c) const { return cut.lead + c * CH; }
+  int held;       // chunks that this thread has
+  int first;      // index in the row of its first chunk; the next ones are T chunks apart each
 
   __device__ __forceinline__ void load(const typename E::bits* row, const RowCut& rc, int part, int part_chunks) {
-    cut = rc;
-    c0 = part * part_chunks;
-    c1 = min(c0 + part_chunks, rc.chunks);
+    const int t = threadIdx.x, c0 = part * part_chunks;
+    held = (min(part_chunks, rc.chunks - c0) - t + T - 1) / T;
+    first = rc.lead + (c0 + t) * CH;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       w[v] = all_neg_inf<E>();
-      if (chunk(v) < c1) w[v] = load16<E>(row + first(chunk(v)));
+      if (v < held) w[v] = load16<E>(row, first + v * (T * CH));
     }
     edge = kNegInf;
     edge_at = -1;
     if (part == 0) {
-      const int t = threadIdx.x, behind = first(rc.chunks) + t - CH;
+      const int behind = rc.lead + rc.chunks * CH + t - CH;
       if (t < rc.lead) edge_at = t;
       else if (t >= CH && behind < rc.V) edge_at = behind;
       if (edge_at >= 0) edge = E::widen(row[edge_at]);
     }
+  }
+
+  // Makes the chunks opaque to the compiler, so that the next pass over them widens them, compares
+  // and computes addresses again: otherwise it keeps one pass's floats, masks and addresses for the
+  // next, more registers than the row itself.
+  __device__ __forceinline__ void forget() {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) asm volatile("" : "+v"(w[v].x), "+v"(w[v].y), "+v"(w[v].z), "+v"(w[v].w));
+    asm volatile("" : "+v"(held), "+v"(first));
   }
 
   // f(value) of every element that the thread holds; -inf for the places it does not fill.
@@ -155,9 +165,9 @@ struct Part {
   __device__ __forceinline__ void each(F f) const {
 #pragma unroll
     for (int v = 0; v < NV; ++v)
-      if (chunk(v) < c1) {
+      if (v < held) {
 #pragma unroll
-        for (int i = 0; i < CH; ++i) f(element<E>(w[v], i), first(chunk(v)) + i);
+        for (int i = 0; i < CH; ++i) f(element<E>(w[v], i), first + v * (T * CH) + i);
       }
     if (edge_at >= 0) f(edge, edge_at);
   }
@@ -204,7 +214,7 @@ struct Part {
   __device__ __forceinline__ void store(typename E::bits* row, F g) const {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      if (chunk(v) >= c1) continue;
+      if (v >= held) continue;
       uint4 o;
       if constexpr (CH == 4) {
         o = make_uint4(E::narrow(g(element<E>(w[v], 0))), E::narrow(g(element<E>(w[v], 1))),
@@ -215,7 +225,7 @@ struct Part {
                        E::to_word(g(element<E>(w[v], 4)), g(element<E>(w[v], 5))),
                        E::to_word(g(element<E>(w[v], 6)), g(element<E>(w[v], 7))));
       }
-      store16<E>(row + first(chunk(v)), o);
+      store16<E>(row, first + v * (T * CH), o);
     }
     if (edge_at >= 0) row[edge_at] = E::narrow(g(edge));
   }
@@ -286,8 +296,19 @@ inline Shape shape_of(int64_t rows, int64_t V, int per_chunk) {
   return s;
 }
 
-inline unsigned grid_of(int64_t units) {  // workgroups walk what is left over
-  return static_cast<unsigned>(units < (int64_t{1} << 22) ? units : (int64_t{1} << 22));
+// Waves per SIMD that the compiler keeps registers for: three workgroups of 512 threads to a CU (80
+// registers), so that one's reductions and searches hide behind another's loads; one of 1024 (128).
+constexpr int min_waves(int threads) { return threads == 1024 ? 4 : 6; }
+
+// One workgroup per unit (a row or a part of one), not a loop over units: what a loop body of this
+// size keeps in registers across units costs the kernels half their occupancy. A grid has fewer than
+// 2^32 threads in x.
+inline dim3 grid_of(int64_t units) {
+  const int64_t x = units < (int64_t{1} << 21) ? units : (int64_t{1} << 21);
+  return dim3(static_cast<unsigned>(x), static_cast<unsigned>((units + x - 1) / x));
+}
+__device__ __forceinline__ int64_t unit_of_block() {
+  return static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x;
 }
 
 // f(element type, threads, chunks held) for a launch's type and shape.

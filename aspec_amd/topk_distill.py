@@ -1,0 +1,201 @@
+"""Distillation from a teacher of which only the best tokens were kept, on the HIP kernels of
+csrc/topk_distill.hip and csrc/topk_distill_fused.hip.
+
+The full-vocabulary losses (`aspec_amd.loss`, the reference's `_prediction_terms`,
+aspec/models/dspark.py:553-612) need the teacher's logits [rows, V]. A cache keeps K pairs (token,
+log-probability) of a teacher row instead, as `aspec_amd.token_logprobs.token_logprobs(top_k=K)`
+writes them, and the divergence is taken over those tokens:
+
+  p = softmax(logits / temperature), q = the teacher's kept probabilities, r = its mass outside them,
+  R = the student's mass outside them
+  tail="bucket":       kl = sum q (log q - log p) + r (log r - log R): the tokens outside as one event
+                       (a lower bound of the full divergence, exact as r goes to 0)
+  tail="renormalize":  kl = sum q' (log q' - log p), q' = q / sum q
+  accept_rate = sum min(p, q) + min(r, R): the probability that a token drafted from p is accepted
+                by the teacher (1 - l1 / 2 of the full losses; an upper bound in the bucket)
+  ce = cross-entropy of the hard target at temperature 1
+
+No reference function matches. No CPU path: the HIP library runs or the call raises.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from aspec_amd import _lib, _timing
+from aspec_amd.loss import IndexCheck
+from aspec_amd.token_logprobs import check_temperature, index_flags, logit_rows, row_stride, settle
+
+_TAILS = {"bucket": 0, "renormalize": 1}
+
+
+class _Call:
+    """The checked arguments of one call: what the forward, the gradient and the one-pass entry share."""
+
+    def __init__(self, logits, targets, teacher_indices, teacher_logprobs, teacher_rows, tail, temperature,
+                 ignore_index):
+        self.temperature = check_temperature(temperature)
+        if tail not in _TAILS:
+            raise ValueError(f"tail must be 'bucket' or 'renormalize', got {tail!r}")
+        self.renormalize = _TAILS[tail]
+        self.ignore_index = int(ignore_index)
+        lead, dev = logits.shape[:-1], logits.device
+        rows = logits.numel() // max(logits.shape[-1] if logits.ndim else 0, 1)
+        if targets is not None:
+            if targets.dtype != torch.int64 or targets.numel() != rows or targets.device != dev:
+                raise ValueError("targets must be one int64 class index per logit row on the logits device")
+            targets = targets.reshape(-1).contiguous()
+        if teacher_logprobs.requires_grad:
+            raise ValueError("top-logit distillation requires a frozen teacher")
+        if (teacher_indices.dtype not in (torch.int64, torch.int32) or teacher_logprobs.dtype != torch.float32
+                or teacher_indices.ndim < 1 or teacher_indices.shape != teacher_logprobs.shape
+                or teacher_indices.shape[-1] == 0
+                or teacher_indices.device != dev or teacher_logprobs.device != dev):
+            raise ValueError("a teacher is int64 or int32 tokens and FP32 log-probabilities of one shape "
+                             "[..., K >= 1] on the logits device")
+        kept = teacher_indices.shape[-1]
+        if teacher_rows is not None:
+            if (teacher_indices.ndim != 2 or (teacher_indices.shape[0] == 0 and rows)
+                    or teacher_rows.dtype != torch.int64 or teacher_rows.numel() != rows or teacher_rows.device != dev):
+                raise ValueError("indexed teacher requires a nonempty 2D table and one int64 index per row "
+                                 "on the logits device")
+            teacher_rows = teacher_rows.reshape(-1).contiguous()
+        elif teacher_indices.shape[:-1] != lead and teacher_indices.shape[:-1] != (rows,):
+            raise ValueError("a teacher without teacher_rows has one row per logit row")
+        self.lead, self.rows, self.kept = lead, rows, kept
+        self.targets, self.teacher_rows = targets, teacher_rows
+        self.indices = teacher_indices.reshape(-1, kept).contiguous()
+        self.logprobs = teacher_logprobs.reshape(-1, kept).contiguous()
+
+    def tensors(self):
+        return self.targets, self.indices, self.logprobs, self.teacher_rows
+
+    @staticmethod
+    def of_logits(flat):
+        return (flat.data_ptr(), _lib.mask_dtype_code(flat), flat.shape[0], flat.shape[1], row_stride(flat))
+
+    def of_teacher(self):
+        return (_lib.ptr(self.targets), self.ignore_index, self.indices.data_ptr(), _lib.mask_dtype_code(self.indices),
+                self.logprobs.data_ptr(), self.kept, _lib.ptr(self.teacher_rows), self.indices.shape[0])
+
+    def outputs(self, flat, want_argmax, check):
+        """(ce, kl, accept_rate, argmax, stats, workspace, flags) to be written."""
+        lib, dev = _lib.load(), flat.device
+        size = ctypes.c_size_t()
+        _lib.check(lib.aspec_topk_distill_workspace_bytes(_lib.mask_dtype_code(flat), *flat.shape, ctypes.byref(size)))
+
+        def empty(dtype=torch.float32):
+            return torch.empty(self.lead, dtype=dtype, device=dev)
+
+        return (empty() if self.targets is not None else None, empty(), empty(),
+                empty(torch.int64) if want_argmax else None,
+                torch.empty((self.rows, lib.aspec_topk_distill_stats_floats()), dtype=torch.float32, device=dev),
+                torch.empty(size.value, dtype=torch.uint8, device=dev) if size.value else None,
+                index_flags(check, dev))
+
+
+class _TopkDistill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, call, want_argmax, check, has_backward):
+        flat = logit_rows(logits, "top-logit distillation")
+        dev = flat.device
+        with torch.cuda.device(dev):
+            ce, kl, accept, amax, stats, workspace, flags = call.outputs(flat, want_argmax, check)
+            with _timing.region("topk_distill_fwd"):
+                _lib.call("aspec_topk_distill_fwd", *call.of_logits(flat), *call.of_teacher(), call.renormalize,
+                          call.temperature, *map(_lib.ptr, (ce, kl, accept, amax, stats, workspace, flags)),
+                          _lib.stream_handle(dev))
+            ctx.check = None if flags is None else IndexCheck(flags)
+        if not has_backward:
+            settle(ctx.check)
+        ctx.save_for_backward(flat, stats, *call.tensors())
+        ctx.call, ctx.shape = call, logits.shape
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(*(t for t in (accept, amax) if t is not None))
+        return ce, kl, accept, amax
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_ce, g_kl, *_):
+        flat, stats = ctx.saved_tensors[:2]  # unpacking also checks that no input was changed in place
+        call, dev = ctx.call, flat.device
+        grads = [None if g is None else g.to(torch.float32).contiguous() for g in (g_ce, g_kl)]
+        grad = torch.empty(flat.shape, dtype=flat.dtype, device=dev)
+        with torch.cuda.device(dev), _timing.region("topk_distill_bwd"):
+            _lib.call("aspec_topk_distill_bwd", *call.of_logits(flat), *call.of_teacher(), call.temperature,
+                      stats.data_ptr(), *map(_lib.ptr, grads), grad.data_ptr(), flat.shape[1],
+                      _lib.stream_handle(dev))
+        # the forward's flag, read with this backward's kernel already queued
+        settle(ctx.check)
+        return grad.view(ctx.shape), None, None, None, None
+
+
+def topk_distill_from_logits(logits, targets, teacher_indices, teacher_logprobs, *, teacher_rows=None, tail="bucket",
+                             temperature=1.0, ignore_index=-100, return_argmax=False, check_indices=True):
+    """Per-row fp32 (ce, kl, accept_rate[, argmax]) of logits [..., V] (bf16, fp16 or fp32, V <= 524288)
+    in one read; `ce` and `kl` are differentiable in `logits` (one read and one write).
+
+    `targets` [...] int64 (`ignore_index`: ce 0, no gradient) or None (ce is None).
+    `teacher_indices` (int64 or int32) and `teacher_logprobs` (fp32) [..., K], K <= 128, hold a frozen
+    teacher's kept tokens and their log-probabilities at `temperature`, in any order, each token once;
+    index -1 is an unused slot. With `teacher_rows` [...] int64 they are a [T, K] table addressed per
+    row. A row without any token has kl 0, accept_rate 0 and no gradient of kl. In the bucket a
+    remaining mass up to 2^-20 counts as the rounding of the log-probabilities, that is as none.
+
+    Logits of -inf are tokens without probability: a kept one, or a whole tail that the teacher gives
+    mass, makes kl infinite, as the definition has it, with finite gradients. A row of nothing else
+    has infinite losses and a zero gradient; one with a NaN or +inf has NaN.
+
+    A target, teacher token or teacher row out of range, or a token twice in a row, gives a NaN row
+    (losses and gradient; a bad target: ce and gradient) and raises ValueError: before the call
+    returns, or, where `logits` requires grad, from the backward, behind its kernel. Reading that
+    check waits for the GPU: with `check_indices=False` nothing waits, and the NaN is the only sign.
+    So it is in a call that is captured into a graph."""
+    call = _Call(logits, targets, teacher_indices, teacher_logprobs, teacher_rows, tail, temperature, ignore_index)
+    out = _TopkDistill.apply(logits, call, return_argmax, check_indices,
+                             torch.is_grad_enabled() and logits.requires_grad)
+    return out if return_argmax else out[:3]
+
+
+def topk_distill_fused_grad(logits, targets, teacher_indices, teacher_logprobs, *, ce_weights=None, kl_weights,
+                            teacher_rows=None, tail="bucket", temperature=1.0, ignore_index=-100, return_argmax=False,
+                            in_place=False, check_indices=True):
+    """`topk_distill_from_logits` and dlogits of sum_r (ce_weights[r] ce[r] + kl_weights[r] kl[r]) from
+    one read of the logits (no autograd): (ce, kl, accept_rate, dlogits[, argmax]). `ce_weights` goes
+    with `targets`. With `in_place` the dlogits overwrite `logits`, which then are rows of adjacent
+    elements. Rows too long for one workgroup (V > 163840, fp32: 81920) are read twice."""
+    out, check = _fused(logits, targets, teacher_indices, teacher_logprobs, ce_weights, kl_weights, teacher_rows, tail,
+                        temperature, ignore_index, return_argmax, in_place, check_indices)
+    settle(check)
+    return out if return_argmax else out[:4]
+
+
+def _fused(logits, targets, teacher_indices, teacher_logprobs, ce_weights, kl_weights, teacher_rows, tail, temperature,
+           ignore_index, return_argmax, in_place, check_indices):
+    """The launch behind `topk_distill_fused_grad`, its index check still to be read."""
+    call = _Call(logits, targets, teacher_indices, teacher_logprobs, teacher_rows, tail, temperature, ignore_index)
+    if (targets is None) != (ce_weights is None):
+        raise ValueError("ce_weights go with targets")
+    weights = []
+    for w in (ce_weights, kl_weights):
+        if w is not None and (w.numel() != call.rows or w.device != logits.device):
+            raise ValueError("objective weights must hold one value per logit row on the logits device")
+        weights.append(None if w is None else w.detach().reshape(-1).to(torch.float32).contiguous())
+    logits = logits.detach()
+    flat = logit_rows(logits, "top-logit distillation")
+    if in_place and flat.data_ptr() != logits.data_ptr():
+        raise ValueError("in_place needs logits whose rows are evenly spaced and their elements adjacent")
+    dev = flat.device
+    with torch.cuda.device(dev):
+        ce, kl, accept, amax, stats, workspace, flags = call.outputs(flat, return_argmax, check_indices)
+        grad = flat if in_place else torch.empty(flat.shape, dtype=flat.dtype, device=dev)
+        with _timing.region("topk_distill_fused"):
+            _lib.call("aspec_topk_distill_fused_fwd_bwd", *call.of_logits(flat), *call.of_teacher(), call.renormalize,
+                      call.temperature, *map(_lib.ptr, weights),
+                      *map(_lib.ptr, (ce, kl, accept, amax, stats, workspace)), grad.data_ptr(), row_stride(grad),
+                      _lib.ptr(flags), _lib.stream_handle(dev))
+        check = None if flags is None else IndexCheck(flags)
+    return (ce, kl, accept, logits if in_place else grad.view(logits.shape), amax), check

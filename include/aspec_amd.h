@@ -401,6 +401,57 @@ int aspec_token_logprobs_bwd(const void* logits, int dtype, int64_t rows, int64_
                              const float* grad_entropy, const float* grad_top, void* grad_logits,
                              int64_t grad_stride, void* stream);
 
+/*
+ * Distillation from a teacher of which only the best tokens were kept. No counterpart in the
+ * reference, whose losses take the teacher's logits whole (aspec/models/dspark.py:553-612).
+ *
+ * logits as for aspec_token_logprobs_fwd. teacher_tokens (token_dtype ASPEC_MASK_I64 or
+ * ASPEC_MASK_I32; -1: an unused slot) and teacher_logprobs [num_teacher_rows][kept], kept <= 128;
+ * teacher_rows [rows] addresses them per row (NULL: row r is teacher row r). With
+ * p = softmax(logits / temperature) and q = exp(teacher_logprobs) of the used slots:
+ *   renormalize = 0: r = 1 - sum q (0 where it is at most 2^-20), R = the sum of p over the tokens that
+ *     were not kept, kl = sum q (log q - log p) + r (log r - log R), accept = sum min(p, q) + min(r, R)
+ *   renormalize = 1: q scaled to sum 1, kl = sum q (log q - log p), accept = sum min(p, q)
+ *   ce (with targets; both may be NULL): cross-entropy of the target at temperature 1; 0 for ignore_index
+ *   argmax (may be NULL): the row's largest logit, NaN above everything, ties to the lower index
+ *   stats: aspec_topk_distill_stats_floats() floats per row, for the gradient.
+ * A row without a used slot: kl 0, accept 0. Bits of *status_flags (caller-zeroed, may be NULL), with
+ * NaN rows: 1 a teacher row out of range, 2 a target out of range, 8 a teacher token out of range, 16
+ * a teacher token twice in a row. workspace: of aspec_topk_distill_workspace_bytes (0 for most
+ * shapes; uninitialised; free once the call's kernels are done).
+ *
+ * aspec_topk_distill_bwd writes the gradient of sum (grad_ce ce + grad_kl kl) (each may be NULL) in
+ * the logits' dtype to grad_logits [rows][grad_stride], from the same teacher and the forward's
+ * stats. aspec_topk_distill_fused_fwd_bwd is both in one call, the logits read once up to 163840 (fp32:
+ * 81920) to a row. grad_logits may be the logits' own buffer, with their row stride.
+ */
+int aspec_topk_distill_stats_floats(void);
+int aspec_topk_distill_workspace_bytes(int dtype, int64_t rows, int64_t vocab, size_t* bytes);
+int aspec_topk_distill_fwd(const void* logits, int dtype, int64_t rows, int64_t vocab,
+                           int64_t row_stride, const int64_t* targets, int64_t ignore_index,
+                           const void* teacher_tokens, int token_dtype,
+                           const float* teacher_logprobs, int64_t kept, const int64_t* teacher_rows,
+                           int64_t num_teacher_rows, int renormalize, float temperature, float* ce,
+                           float* kl, float* accept, int64_t* argmax, float* stats, void* workspace,
+                           int32_t* status_flags, void* stream);
+int aspec_topk_distill_bwd(const void* logits, int dtype, int64_t rows, int64_t vocab,
+                           int64_t row_stride, const int64_t* targets, int64_t ignore_index,
+                           const void* teacher_tokens, int token_dtype,
+                           const float* teacher_logprobs, int64_t kept, const int64_t* teacher_rows,
+                           int64_t num_teacher_rows, float temperature, const float* stats,
+                           const float* grad_ce, const float* grad_kl, void* grad_logits,
+                           int64_t grad_stride, void* stream);
+int aspec_topk_distill_fused_fwd_bwd(const void* logits, int dtype, int64_t rows, int64_t vocab,
+                                     int64_t row_stride, const int64_t* targets, int64_t ignore_index,
+                                     const void* teacher_tokens, int token_dtype,
+                                     const float* teacher_logprobs, int64_t kept,
+                                     const int64_t* teacher_rows, int64_t num_teacher_rows,
+                                     int renormalize, float temperature, const float* grad_ce,
+                                     const float* grad_kl, float* ce, float* kl, float* accept,
+                                     int64_t* argmax, float* stats, void* workspace,
+                                     void* grad_logits, int64_t grad_stride, int32_t* status_flags,
+                                     void* stream);
+
 /* ---------------------------------------------------------------------------------------------
  * Row-level operations around the attention and loss: packing, anchors, output blocks, targets.
  * ------------------------------------------------------------------------------------------- */
