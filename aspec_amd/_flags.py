@@ -1,0 +1,79 @@
+"""Index errors of a launch, reported through pinned host memory.
+
+A kernel that meets an index it cannot compute with writes NaN and sets a word here: a plain store,
+which only a bad index ever makes, so a launch needs no device flag to be cleared before it and
+copied after it, just an event behind it. The words go back to a pool when their owner is dropped, and
+are handed out again once their event has passed: a launch whose owner is gone may still write.
+"""
+
+from __future__ import annotations
+
+import contextlib
+from collections import defaultdict, deque
+
+import torch
+
+# the words, in the order of include/aspec_amd.h
+_MESSAGES = (
+    "teacher index out of range: every target index must address a row of the teacher table",
+    "cross-entropy target out of range: targets must lie in [0, vocab) or equal ignore_index",
+    "token id out of range: token ids must lie in [0, vocab) or equal ignore_index",
+    "teacher token out of range: a teacher row's tokens must lie in [0, vocab), or be -1 for an unused slot",
+    "teacher token repeated: a teacher row's tokens must be distinct",
+)
+_pool = defaultdict(deque)
+
+
+class IndexFlags:
+    """The words of one launch on `device`: `ptr` goes to the kernel, `record` follows the launch on its
+    stream, `raise_if_bad` waits for it and raises ValueError where an index was bad."""
+
+    def __init__(self, device: torch.device):
+        self._home = _pool[device.index]
+        self._slot = None
+        for _ in range(min(2, len(self._home))):  # the oldest first; one still pending goes to the end
+            with contextlib.suppress(IndexError):
+                slot = self._home.popleft()
+                if slot[2].query():
+                    self._slot = slot
+                    break
+                self._home.append(slot)
+        if self._slot is None:
+            words = torch.zeros(len(_MESSAGES), dtype=torch.int32, pin_memory=True)
+            self._slot = (words, words.numpy(), torch.cuda.Event())
+        self._slot[1][:] = 0
+
+    @property
+    def ptr(self) -> int:
+        return self._slot[0].data_ptr()
+
+    def record(self, stream: torch.cuda.Stream) -> None:
+        self._slot[2].record(stream)
+
+    def raise_if_bad(self) -> None:
+        self._slot[2].synchronize()
+        if self._slot[1].any():
+            raise ValueError(_MESSAGES[int(self._slot[1].argmax())])
+
+    def __del__(self):
+        if self._slot is not None:
+            self._home.append(self._slot)
+
+
+def index_flags(wanted: bool, device: torch.device) -> IndexFlags | None:
+    """The flags of a launch whose indices are to be checked. None where nothing can read them: the
+    caller wants no check, or the launch is captured into a graph, whose replays no host follows."""
+    if not wanted or torch.cuda.is_current_stream_capturing():
+        return None
+    return IndexFlags(device)
+
+
+def settle(flags: IndexFlags | None) -> None:
+    """Reads a deferred check behind the launches that it was deferred for."""
+    if flags is not None and not torch.cuda.is_current_stream_capturing():
+        flags.raise_if_bad()
+
+
+def on_device(device: torch.device):
+    """`device` as the current one, where it is not already."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)

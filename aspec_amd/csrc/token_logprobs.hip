@@ -41,7 +41,7 @@ struct FwdArgs {
   float* stats;
   float* part_sums;   // [rows][parts][3]: maximum, S, D
   uint64_t* part_top; // [rows][parts][K], descending, 0 behind a part's last token
-  int32_t* flags;
+  int32_t* status;
 };
 
 struct BwdArgs {
@@ -97,14 +97,15 @@ __device__ __forceinline__ RowResult finish_row(const FwdArgs& a, int64_t row, c
   if (writer) {
     const float entropy = empty ? 0.f : log_s - kLn2 * s.D / s.S;
     a.entropy[row] = entropy;
-    *reinterpret_cast<float4*>(a.stats + row * kStats) = make_float4(s.m, s.S, entropy, empty ? 0.f : s.D / s.S);
+    if (a.stats)
+      *reinterpret_cast<float4*>(a.stats + row * kStats) = make_float4(s.m, s.S, entropy, empty ? 0.f : s.D / s.S);
     if (a.ids) {
       float lp = 0.f;
       if (id != a.ignore_index) {
         lp = r.logprob(at_id);
         if (id < 0 || id >= a.V) {
           lp = __builtin_nanf("");
-          if (a.flags) atomicOr(a.flags, 4);
+          report(a.status, kBadTokenId);
         }
       }
       a.logprobs[row] = lp;
@@ -497,11 +498,11 @@ extern "C" int aspec_token_logprobs_fwd(const void* logits, int dtype, int64_t r
                                         int64_t row_stride, const int64_t* token_ids, int64_t ignore_index,
                                         float temperature, int64_t top_k, float* logprobs, float* entropy,
                                         float* top_logprobs, int64_t* top_indices, float* stats,
-                                        void* workspace, int32_t* status_flags, void* stream) {
+                                        void* workspace, int32_t* status_words, void* stream) {
   if (const int e = check_rows(dtype, rows, vocab, row_stride, temperature, top_k)) return e;
   if (rows == 0) return ASPEC_OK;
   const vocab::Shape s = vocab::shape_of(rows, vocab, vocab::per_chunk_of(dtype));
-  if (!logits || !entropy || !stats || (token_ids && !logprobs) || (top_k && (!top_logprobs || !top_indices)) ||
+  if (!logits || !entropy || (token_ids && !logprobs) || (top_k && (!top_logprobs || !top_indices)) ||
       (s.parts > 1 && !workspace))
     return set_error(ASPEC_ERR_INVALID, "null pointer passed to token log-probabilities");
   FwdArgs a{};
@@ -522,7 +523,7 @@ extern "C" int aspec_token_logprobs_fwd(const void* logits, int dtype, int64_t r
   a.stats = stats;
   a.part_top = static_cast<uint64_t*>(workspace);
   a.part_sums = reinterpret_cast<float*>(a.part_top + rows * s.parts * top_k);
-  a.flags = status_flags;
+  a.status = status_words;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   dispatch(dtype, s, [&](auto e, auto t, auto nv) { launch_fwd<decltype(e), t.value, nv.value>(a, st); });
   return check_launch("token_logprobs_kernel");

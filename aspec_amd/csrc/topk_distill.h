@@ -31,8 +31,6 @@ using namespace vocab;
 constexpr int kStats = 8;  // per row: M, S, tail maximum, tail sum, r, c, sum q + r, S at temperature 1
 constexpr double kNoTail = 0x1p-20;
 
-enum Flag { kBadTeacherRow = 1, kBadTarget = 2, kBadToken = 8, kRepeated = 16 };
-
 // exp and log of the K-term sums in 64 bits: what the library's do in fewer registers (the kernels
 // hold a row in theirs).
 // exp(x) = 2^k exp(x - k ln2), |x - k ln2| <= 0.35: its series to the 10th power leaves 2e-13.
@@ -68,10 +66,10 @@ struct Args {
   float* kl;
   float* accept;
   int64_t* argmax;         // may be null
-  float* stats;
+  float* stats;            // the forward's may be null
   float* part_sums;        // [rows][parts][4]: tail maximum, S, S1
   uint64_t* part_arg;      // [rows][parts]
-  int32_t* flags;          // may be null
+  int32_t* status;         // may be null
   const float* g_ce;       // may be null
   const float* g_kl;       // may be null
   void* dx;
@@ -88,10 +86,6 @@ struct Kept {
   double q[kMaxTop];   // exp(lp); 0 for an unused slot
   int poison;          // an index that the row cannot be computed with
 };
-
-__device__ __forceinline__ void raise(const Args& a, int flag) {
-  if (a.flags) atomicOr(a.flags, flag);
-}
 
 // The teacher's row, or -1.
 __device__ __forceinline__ int64_t teacher_row(const Args& a, int64_t row) {
@@ -272,13 +266,15 @@ __device__ __forceinline__ void finish_row(const Args& a, int64_t row, int lane,
       if (target.token >= 0) ce = empty ? INFINITY : static_cast<float>(log64(S1) - static_cast<double>(x_target - base));
       if (target.bad) {
         ce = __builtin_nanf("");
-        raise(a, kBadTarget);
+        report(a.status, kBadTarget);
       }
       a.ce[row] = ce;
     }
-    float4* o = reinterpret_cast<float4*>(a.stats + row * kStats);
-    o[0] = make_float4(st[0], st[1], st[2], st[3]);
-    o[1] = make_float4(st[4], st[5], st[6], st[7]);
+    if (a.stats) {
+      float4* o = reinterpret_cast<float4*>(a.stats + row * kStats);
+      o[0] = make_float4(st[0], st[1], st[2], st[3]);
+      o[1] = make_float4(st[4], st[5], st[6], st[7]);
+    }
   }
 }
 
@@ -326,7 +322,7 @@ __device__ __forceinline__ void forward_unit(const Args& a, int64_t unit, Kept<T
     if (trow < 0 || __any(bad)) {
       if (lane == 0) {
         kept.poison = 1;
-        raise(a, trow < 0 ? kBadTeacherRow : kBadToken);
+        report(a.status, trow < 0 ? kBadTeacherRow : kBadTeacherToken);
       }
     }
   }
@@ -338,7 +334,7 @@ __device__ __forceinline__ void forward_unit(const Args& a, int64_t unit, Kept<T
     for (int j = kept.next[k]; j >= 0; j = kept.next[j])
       if (kept.token[j] == kept.token[k]) {
         kept.poison = 1;
-        raise(a, kRepeated);
+        report(a.status, kRepeatedToken);
       }
   }
   // ---- the tail's maximum and sums

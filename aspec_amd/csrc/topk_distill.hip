@@ -165,7 +165,7 @@ Args make_args(const void* logits, int dtype, int64_t rows, int64_t vocab, int64
                const int64_t* targets, int64_t ignore_index, const void* tokens, int token_dtype,
                const float* logprobs, int64_t kept, const int64_t* teacher_rows, int64_t num_teacher_rows,
                int renormalize, float temperature, float* ce, float* kl, float* accept, int64_t* argmax, float* stats,
-               void* workspace, int32_t* flags) {
+               void* workspace, int32_t* status) {
   const Shape s = shape_of(rows, vocab, per_chunk_of(dtype));
   Args a{};
   a.x = logits;
@@ -191,7 +191,7 @@ Args make_args(const void* logits, int dtype, int64_t rows, int64_t vocab, int64
   a.stats = stats;
   a.part_sums = static_cast<float*>(workspace);
   a.part_arg = reinterpret_cast<uint64_t*>(a.part_sums + rows * s.parts * 4);
-  a.flags = flags;
+  a.status = status;
   return a;
 }
 
@@ -229,13 +229,13 @@ extern "C" int aspec_topk_distill_fwd(const void* logits, int dtype, int64_t row
                                       int token_dtype, const float* teacher_logprobs, int64_t kept,
                                       const int64_t* teacher_rows, int64_t num_teacher_rows, int renormalize,
                                       float temperature, float* ce, float* kl, float* accept, int64_t* argmax,
-                                      float* stats, void* workspace, int32_t* status_flags, void* stream) {
+                                      float* stats, void* workspace, int32_t* status_words, void* stream) {
   if (const int e = check_distill(dtype, rows, vocab, row_stride, token_dtype, kept, temperature)) return e;
   if (rows == 0) return ASPEC_OK;
   const Args a = make_args(logits, dtype, rows, vocab, row_stride, targets, ignore_index, teacher_tokens, token_dtype,
                            teacher_logprobs, kept, teacher_rows, num_teacher_rows, renormalize, temperature, ce, kl,
-                           accept, argmax, stats, workspace, status_flags);
-  if (!logits || !teacher_tokens || !teacher_logprobs || (targets && !ce) || !kl || !accept || !stats ||
+                           accept, argmax, stats, workspace, status_words);
+  if (!logits || !teacher_tokens || !teacher_logprobs || (targets && !ce) || !kl || !accept ||
       (a.parts > 1 && !workspace))
     return null_pointer();
   run_fwd(dtype, a, static_cast<hipStream_t>(stream));
@@ -272,21 +272,21 @@ extern "C" int aspec_topk_distill_fused_fwd_bwd(
     int64_t ignore_index, const void* teacher_tokens, int token_dtype, const float* teacher_logprobs, int64_t kept,
     const int64_t* teacher_rows, int64_t num_teacher_rows, int renormalize, float temperature, const float* grad_ce,
     const float* grad_kl, float* ce, float* kl, float* accept, int64_t* argmax, float* stats, void* workspace,
-    void* grad_logits, int64_t grad_stride, int32_t* status_flags, void* stream) {
+    void* grad_logits, int64_t grad_stride, int32_t* status_words, void* stream) {
   if (const int e = check_distill(dtype, rows, vocab, row_stride, token_dtype, kept, temperature)) return e;
   if (grad_stride < vocab)
     return set_error(ASPEC_ERR_INVALID, "top-logit distillation needs a vocabulary and rows at least as far apart");
   if (rows == 0) return ASPEC_OK;
   Args a = make_args(logits, dtype, rows, vocab, row_stride, targets, ignore_index, teacher_tokens, token_dtype,
                      teacher_logprobs, kept, teacher_rows, num_teacher_rows, renormalize, temperature, ce, kl, accept,
-                     argmax, stats, workspace, status_flags);
+                     argmax, stats, workspace, status_words);
   a.g_ce = grad_ce;
   a.g_kl = grad_kl;
   a.dx = grad_logits;
   a.dx_stride = grad_stride;
   const bool fits = topk_distill_fused_fits(vocab, per_chunk_of(dtype));
-  if (!logits || !teacher_tokens || !teacher_logprobs || (targets && !ce) || !kl || !accept || !stats ||
-      !grad_logits || (grad_ce && !targets) || (!fits && a.parts > 1 && !workspace))
+  if (!logits || !teacher_tokens || !teacher_logprobs || (targets && !ce) || !kl || !accept ||
+      !grad_logits || (grad_ce && !targets) || (!fits && (!stats || (a.parts > 1 && !workspace))))
     return null_pointer();
   if (grad_logits == logits && grad_stride != row_stride)
     return set_error(ASPEC_ERR_INVALID, "a gradient in place has the logits' row stride");

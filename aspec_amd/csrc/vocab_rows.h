@@ -25,6 +25,12 @@ constexpr int kMaxTop = 128;     // alternatives per row, teacher tokens per row
 constexpr int kMaxParts = 32;    // workgroups that share one row
 constexpr float kNegInf = -INFINITY;
 
+// The words of status_words, each set to 1 by plain stores: host memory serves as well as the device's.
+enum Status { kBadTeacherRow, kBadTarget, kBadTokenId, kBadTeacherToken, kRepeatedToken };
+__device__ __forceinline__ void report(int32_t* words, Status s) {
+  if (words) __hip_atomic_store(words + s, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+}
+
 // ---- element types -------------------------------------------------------------------------------
 struct Bf16 {
   using bits = uint16_t;

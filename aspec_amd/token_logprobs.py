@@ -18,6 +18,7 @@ or the call raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import NamedTuple, Optional
 
@@ -25,7 +26,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from aspec_amd import _lib, _timing
-from aspec_amd.loss import IndexCheck
+from aspec_amd._flags import index_flags, on_device, settle
 
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
@@ -68,53 +69,50 @@ def check_temperature(temperature) -> float:
     return temperature
 
 
-def index_flags(wanted: bool, device) -> torch.Tensor | None:
-    """The zeroed flag word of a launch whose indices are to be checked. None where nothing can read
-    it: the caller wants no check, or the launch is captured into a graph, whose replays no host
-    follows."""
-    if not wanted or torch.cuda.is_current_stream_capturing():
-        return None
-    return torch.zeros(1, dtype=torch.int32, device=device)
+@functools.lru_cache(maxsize=256)
+def _sizes(dtype: int, rows: int, vocab: int, top_k: int) -> tuple[int, int]:
+    """(workspace bytes, floats of statistics per row) of a call."""
+    lib, size = _lib.load(), ctypes.c_size_t()
+    _lib.check(lib.aspec_token_logprobs_workspace_bytes(dtype, rows, vocab, top_k, ctypes.byref(size)))
+    return size.value, lib.aspec_token_logprobs_stats_floats()
 
 
-def settle(check: IndexCheck | None) -> None:
-    """Reads a deferred check behind the launches that it was deferred for."""
-    if check is not None and not torch.cuda.is_current_stream_capturing():
-        check.raise_if_bad()
+def _forward(logits, ids, top_k, temperature, ignore_index, check_ids, has_backward):
+    """One forward launch: (results, logit rows, statistics, index flags to be settled)."""
+    flat = logit_rows(logits, "token_logprobs")
+    rows, vocab = flat.shape
+    dev, lead = flat.device, logits.shape[:-1]
+    dtype = _lib.mask_dtype_code(flat)
+    work_bytes, stat_floats = _sizes(dtype, rows, vocab, top_k)
+    with on_device(dev):
+        workspace = torch.empty(work_bytes, dtype=torch.uint8, device=dev) if work_bytes else None
+        entropy = torch.empty(lead, dtype=torch.float32, device=dev)
+        logprobs = torch.empty_like(entropy) if ids is not None else None
+        top = torch.empty((*lead, top_k), dtype=torch.float32, device=dev) if top_k else None
+        top_indices = torch.empty((*lead, top_k), dtype=torch.int64, device=dev) if top_k else None
+        stats = torch.empty((rows, stat_floats), dtype=torch.float32, device=dev) if has_backward else None
+        flags = index_flags(check_ids and ids is not None, dev)
+        stream = torch.cuda.current_stream(dev)
+        with _timing.region("token_logprobs_fwd"):
+            _lib.call("aspec_token_logprobs_fwd", flat.data_ptr(), dtype, rows, vocab, row_stride(flat),
+                      _lib.ptr(ids), ignore_index, temperature, top_k, _lib.ptr(logprobs), entropy.data_ptr(),
+                      _lib.ptr(top), _lib.ptr(top_indices), _lib.ptr(stats), _lib.ptr(workspace),
+                      None if flags is None else flags.ptr, stream.cuda_stream)
+        if flags is not None:
+            flags.record(stream)
+    return (logprobs, entropy, top, top_indices), flat, stats, flags
 
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, ids, top_k, temperature, ignore_index, check_ids, has_backward):
-        flat = logit_rows(logits, "token_logprobs")
-        rows, vocab = flat.shape
-        dev, lead = flat.device, logits.shape[:-1]
-        dtype = _lib.mask_dtype_code(flat)
-        lib = _lib.load()
-        with torch.cuda.device(dev):
-            size = ctypes.c_size_t()
-            _lib.check(lib.aspec_token_logprobs_workspace_bytes(dtype, rows, vocab, top_k, ctypes.byref(size)))
-            workspace = torch.empty(size.value, dtype=torch.uint8, device=dev) if size.value else None
-            entropy = torch.empty(lead, dtype=torch.float32, device=dev)
-            logprobs = torch.empty(lead, dtype=torch.float32, device=dev) if ids is not None else None
-            top = torch.empty((*lead, top_k), dtype=torch.float32, device=dev) if top_k else None
-            top_indices = torch.empty((*lead, top_k), dtype=torch.int64, device=dev) if top_k else None
-            stats = torch.empty((rows, lib.aspec_token_logprobs_stats_floats()), dtype=torch.float32, device=dev)
-            flags = index_flags(check_ids and ids is not None, dev)
-            with _timing.region("token_logprobs_fwd"):
-                _lib.call("aspec_token_logprobs_fwd", flat.data_ptr(), dtype, rows, vocab, row_stride(flat),
-                          _lib.ptr(ids), ignore_index, temperature, top_k, _lib.ptr(logprobs),
-                          entropy.data_ptr(), _lib.ptr(top), _lib.ptr(top_indices), stats.data_ptr(),
-                          _lib.ptr(workspace), _lib.ptr(flags), _lib.stream_handle(dev))
-            ctx.check = None if flags is None else IndexCheck(flags)
-        if not has_backward:
-            settle(ctx.check)
-        ctx.save_for_backward(flat, ids, top_indices, stats)
+    def forward(ctx, logits, ids, top_k, temperature, ignore_index, check_ids):
+        out, flat, stats, ctx.flags = _forward(logits, ids, top_k, temperature, ignore_index, check_ids, True)
+        ctx.save_for_backward(flat, ids, out[3], stats)
         ctx.parameters = (top_k, temperature, ignore_index, logits.shape)
         ctx.set_materialize_grads(False)
-        if top_indices is not None:
-            ctx.mark_non_differentiable(top_indices)
-        return logprobs, entropy, top, top_indices
+        if out[3] is not None:
+            ctx.mark_non_differentiable(out[3])
+        return out
 
     @staticmethod
     @once_differentiable
@@ -125,13 +123,13 @@ class _TokenLogprobs(torch.autograd.Function):
         dev = flat.device
         grads = [None if g is None else g.to(torch.float32).contiguous() for g in (g_logprobs, g_entropy, g_top)]
         grad = torch.empty((rows, vocab), dtype=flat.dtype, device=dev)
-        with torch.cuda.device(dev), _timing.region("token_logprobs_bwd"):
+        with on_device(dev), _timing.region("token_logprobs_bwd"):
             _lib.call("aspec_token_logprobs_bwd", flat.data_ptr(), _lib.mask_dtype_code(flat), rows, vocab,
                       row_stride(flat), _lib.ptr(ids), ignore_index, temperature, top_k, _lib.ptr(top_indices),
                       stats.data_ptr(), *map(_lib.ptr, grads), grad.data_ptr(), vocab, _lib.stream_handle(dev))
         # the forward's flag, read with this backward's kernel already queued
-        settle(ctx.check)
-        return grad.view(shape), None, None, None, None, None, None
+        settle(ctx.flags)
+        return grad.view(shape), None, None, None, None, None
 
 
 def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor | None = None, *, top_k: int = 0,
@@ -157,5 +155,9 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor | None = None, 
                 token_ids.shape != logits.shape[:-1] and token_ids.shape != (rows,)):
             raise ValueError("token_ids must be one int64 token per logit row on the logits device")
         token_ids = token_ids.reshape(-1).contiguous()
-    return TokenLogprobs(*_TokenLogprobs.apply(logits, token_ids, int(top_k), temperature, int(ignore_index),
-                                               check_ids, torch.is_grad_enabled() and logits.requires_grad))
+    args = (logits, token_ids, int(top_k), temperature, int(ignore_index), check_ids)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return TokenLogprobs(*_TokenLogprobs.apply(*args))
+    out, _, _, flags = _forward(*args, False)
+    settle(flags)
+    return TokenLogprobs(*out)

@@ -21,13 +21,14 @@ No reference function matches. No CPU path: the HIP library runs or the call rai
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from aspec_amd import _lib, _timing
-from aspec_amd.loss import IndexCheck
-from aspec_amd.token_logprobs import check_temperature, index_flags, logit_rows, row_stride, settle
+from aspec_amd._flags import index_flags, on_device, settle
+from aspec_amd.token_logprobs import check_temperature, logit_rows, row_stride
 
 _TAILS = {"bucket": 0, "renormalize": 1}
 
@@ -81,41 +82,51 @@ class _Call:
         return (_lib.ptr(self.targets), self.ignore_index, self.indices.data_ptr(), _lib.mask_dtype_code(self.indices),
                 self.logprobs.data_ptr(), self.kept, _lib.ptr(self.teacher_rows), self.indices.shape[0])
 
-    def outputs(self, flat, want_argmax, check):
-        """(ce, kl, accept_rate, argmax, stats, workspace, flags) to be written."""
-        lib, dev = _lib.load(), flat.device
-        size = ctypes.c_size_t()
-        _lib.check(lib.aspec_topk_distill_workspace_bytes(_lib.mask_dtype_code(flat), *flat.shape, ctypes.byref(size)))
+    def outputs(self, flat, want_argmax, want_stats):
+        """(ce, kl, accept_rate, argmax, stats, workspace) to be written; None where not wanted."""
+        dev = flat.device
+        work_bytes, stat_floats = _sizes(_lib.mask_dtype_code(flat), *flat.shape)
+        kl = torch.empty(self.lead, dtype=torch.float32, device=dev)
+        return (torch.empty_like(kl) if self.targets is not None else None, kl, torch.empty_like(kl),
+                torch.empty(self.lead, dtype=torch.int64, device=dev) if want_argmax else None,
+                torch.empty((self.rows, stat_floats), dtype=torch.float32, device=dev) if want_stats else None,
+                torch.empty(work_bytes, dtype=torch.uint8, device=dev) if work_bytes else None)
 
-        def empty(dtype=torch.float32):
-            return torch.empty(self.lead, dtype=dtype, device=dev)
 
-        return (empty() if self.targets is not None else None, empty(), empty(),
-                empty(torch.int64) if want_argmax else None,
-                torch.empty((self.rows, lib.aspec_topk_distill_stats_floats()), dtype=torch.float32, device=dev),
-                torch.empty(size.value, dtype=torch.uint8, device=dev) if size.value else None,
-                index_flags(check, dev))
+@functools.lru_cache(maxsize=256)
+def _sizes(dtype: int, rows: int, vocab: int) -> tuple[int, int]:
+    """(workspace bytes, floats of statistics per row) of a call."""
+    lib, size = _lib.load(), ctypes.c_size_t()
+    _lib.check(lib.aspec_topk_distill_workspace_bytes(dtype, rows, vocab, ctypes.byref(size)))
+    return size.value, lib.aspec_topk_distill_stats_floats()
+
+
+def _forward(logits, call, want_argmax, check, has_backward):
+    """One forward launch: (results, logit rows, statistics, index flags to be settled)."""
+    flat = logit_rows(logits, "top-logit distillation")
+    dev = flat.device
+    with on_device(dev):
+        *out, stats, workspace = call.outputs(flat, want_argmax, has_backward)
+        flags = index_flags(check, dev)
+        stream = torch.cuda.current_stream(dev)
+        with _timing.region("topk_distill_fwd"):
+            _lib.call("aspec_topk_distill_fwd", *call.of_logits(flat), *call.of_teacher(), call.renormalize,
+                      call.temperature, *map(_lib.ptr, (*out, stats, workspace)),
+                      None if flags is None else flags.ptr, stream.cuda_stream)
+        if flags is not None:
+            flags.record(stream)
+    return tuple(out), flat, stats, flags
 
 
 class _TopkDistill(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, call, want_argmax, check, has_backward):
-        flat = logit_rows(logits, "top-logit distillation")
-        dev = flat.device
-        with torch.cuda.device(dev):
-            ce, kl, accept, amax, stats, workspace, flags = call.outputs(flat, want_argmax, check)
-            with _timing.region("topk_distill_fwd"):
-                _lib.call("aspec_topk_distill_fwd", *call.of_logits(flat), *call.of_teacher(), call.renormalize,
-                          call.temperature, *map(_lib.ptr, (ce, kl, accept, amax, stats, workspace, flags)),
-                          _lib.stream_handle(dev))
-            ctx.check = None if flags is None else IndexCheck(flags)
-        if not has_backward:
-            settle(ctx.check)
+    def forward(ctx, logits, call, want_argmax, check):
+        out, flat, stats, ctx.flags = _forward(logits, call, want_argmax, check, True)
         ctx.save_for_backward(flat, stats, *call.tensors())
         ctx.call, ctx.shape = call, logits.shape
         ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(*(t for t in (accept, amax) if t is not None))
-        return ce, kl, accept, amax
+        ctx.mark_non_differentiable(*(t for t in out[2:] if t is not None))
+        return out
 
     @staticmethod
     @once_differentiable
@@ -124,13 +135,13 @@ class _TopkDistill(torch.autograd.Function):
         call, dev = ctx.call, flat.device
         grads = [None if g is None else g.to(torch.float32).contiguous() for g in (g_ce, g_kl)]
         grad = torch.empty(flat.shape, dtype=flat.dtype, device=dev)
-        with torch.cuda.device(dev), _timing.region("topk_distill_bwd"):
+        with on_device(dev), _timing.region("topk_distill_bwd"):
             _lib.call("aspec_topk_distill_bwd", *call.of_logits(flat), *call.of_teacher(), call.temperature,
                       stats.data_ptr(), *map(_lib.ptr, grads), grad.data_ptr(), flat.shape[1],
                       _lib.stream_handle(dev))
-        # the forward's flag, read with this backward's kernel already queued
-        settle(ctx.check)
-        return grad.view(ctx.shape), None, None, None, None
+        # the forward's flags, read with this backward's kernel already queued
+        settle(ctx.flags)
+        return grad.view(ctx.shape), None, None, None
 
 
 def topk_distill_from_logits(logits, targets, teacher_indices, teacher_logprobs, *, teacher_rows=None, tail="bucket",
@@ -155,8 +166,11 @@ def topk_distill_from_logits(logits, targets, teacher_indices, teacher_logprobs,
     check waits for the GPU: with `check_indices=False` nothing waits, and the NaN is the only sign.
     So it is in a call that is captured into a graph."""
     call = _Call(logits, targets, teacher_indices, teacher_logprobs, teacher_rows, tail, temperature, ignore_index)
-    out = _TopkDistill.apply(logits, call, return_argmax, check_indices,
-                             torch.is_grad_enabled() and logits.requires_grad)
+    if logits.requires_grad and torch.is_grad_enabled():
+        out = _TopkDistill.apply(logits, call, return_argmax, check_indices)
+    else:
+        out, _, _, flags = _forward(logits, call, return_argmax, check_indices, False)
+        settle(flags)
     return out if return_argmax else out[:3]
 
 
@@ -167,15 +181,15 @@ def topk_distill_fused_grad(logits, targets, teacher_indices, teacher_logprobs, 
     one read of the logits (no autograd): (ce, kl, accept_rate, dlogits[, argmax]). `ce_weights` goes
     with `targets`. With `in_place` the dlogits overwrite `logits`, which then are rows of adjacent
     elements. Rows too long for one workgroup (V > 163840, fp32: 81920) are read twice."""
-    out, check = _fused(logits, targets, teacher_indices, teacher_logprobs, ce_weights, kl_weights, teacher_rows, tail,
+    out, flags = _fused(logits, targets, teacher_indices, teacher_logprobs, ce_weights, kl_weights, teacher_rows, tail,
                         temperature, ignore_index, return_argmax, in_place, check_indices)
-    settle(check)
+    settle(flags)
     return out if return_argmax else out[:4]
 
 
 def _fused(logits, targets, teacher_indices, teacher_logprobs, ce_weights, kl_weights, teacher_rows, tail, temperature,
            ignore_index, return_argmax, in_place, check_indices):
-    """The launch behind `topk_distill_fused_grad`, its index check still to be read."""
+    """The launch behind `topk_distill_fused_grad`, its index flags still to be settled."""
     call = _Call(logits, targets, teacher_indices, teacher_logprobs, teacher_rows, tail, temperature, ignore_index)
     if (targets is None) != (ce_weights is None):
         raise ValueError("ce_weights go with targets")
@@ -189,13 +203,16 @@ def _fused(logits, targets, teacher_indices, teacher_logprobs, ce_weights, kl_we
     if in_place and flat.data_ptr() != logits.data_ptr():
         raise ValueError("in_place needs logits whose rows are evenly spaced and their elements adjacent")
     dev = flat.device
-    with torch.cuda.device(dev):
-        ce, kl, accept, amax, stats, workspace, flags = call.outputs(flat, return_argmax, check_indices)
+    with on_device(dev):
+        ce, kl, accept, amax, stats, workspace = call.outputs(flat, return_argmax, True)
         grad = flat if in_place else torch.empty(flat.shape, dtype=flat.dtype, device=dev)
+        flags = index_flags(check_indices, dev)
+        stream = torch.cuda.current_stream(dev)
         with _timing.region("topk_distill_fused"):
             _lib.call("aspec_topk_distill_fused_fwd_bwd", *call.of_logits(flat), *call.of_teacher(), call.renormalize,
                       call.temperature, *map(_lib.ptr, weights),
                       *map(_lib.ptr, (ce, kl, accept, amax, stats, workspace)), grad.data_ptr(), row_stride(grad),
-                      _lib.ptr(flags), _lib.stream_handle(dev))
-        check = None if flags is None else IndexCheck(flags)
-    return (ce, kl, accept, logits if in_place else grad.view(logits.shape), amax), check
+                      None if flags is None else flags.ptr, stream.cuda_stream)
+        if flags is not None:
+            flags.record(stream)
+    return (ce, kl, accept, logits if in_place else grad.view(logits.shape), amax), flags

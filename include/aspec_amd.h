@@ -372,12 +372,13 @@ int aspec_sampled_l1_bwd(const void* logits, const void* teacher, const int64_t*
  *
  * logits [rows][row_stride >= vocab] of dtype ASPEC_MASK_BF16, ASPEC_MASK_F16 or ASPEC_MASK_F32,
  * vocab <= 524288, any element alignment. With logp = log_softmax(logits / temperature):
- *   logprobs[r] = logp[token_ids[r]]; 0 for ignore_index; NaN, and bit 4 of *status_flags (caller-
- *     zeroed, may be NULL), for a token outside [0, vocab). token_ids and logprobs may be NULL.
+ *   logprobs[r] = logp[token_ids[r]]; 0 for ignore_index; NaN, and status_words[2] = 1, for a token
+ *     outside [0, vocab). token_ids and logprobs may be NULL.
  *   entropy[r] = -sum p logp
  *   top_logprobs / top_indices [rows][top_k] (top_k <= 128 and vocab; NULL with top_k 0): by logit,
  *     descending, ties by the lower index, NaN above everything.
- *   stats: aspec_token_logprobs_stats_floats() floats per row, for the backward.
+ *   stats: aspec_token_logprobs_stats_floats() floats per row, for the backward (NULL: none follows).
+ *   status_words: 5 int32 that the caller has zeroed, in device or pinned host memory, or NULL.
  * A row of -inf alone: logprobs -inf, entropy 0, no gradient. workspace: of
  * aspec_token_logprobs_workspace_bytes (0 for most shapes; uninitialised; free once the call's
  * kernels are done).
@@ -393,7 +394,7 @@ int aspec_token_logprobs_fwd(const void* logits, int dtype, int64_t rows, int64_
                              int64_t row_stride, const int64_t* token_ids, int64_t ignore_index,
                              float temperature, int64_t top_k, float* logprobs, float* entropy,
                              float* top_logprobs, int64_t* top_indices, float* stats, void* workspace,
-                             int32_t* status_flags, void* stream);
+                             int32_t* status_words, void* stream);
 int aspec_token_logprobs_bwd(const void* logits, int dtype, int64_t rows, int64_t vocab,
                              int64_t row_stride, const int64_t* token_ids, int64_t ignore_index,
                              float temperature, int64_t top_k, const int64_t* top_indices,
@@ -414,10 +415,10 @@ int aspec_token_logprobs_bwd(const void* logits, int dtype, int64_t rows, int64_
  *   renormalize = 1: q scaled to sum 1, kl = sum q (log q - log p), accept = sum min(p, q)
  *   ce (with targets; both may be NULL): cross-entropy of the target at temperature 1; 0 for ignore_index
  *   argmax (may be NULL): the row's largest logit, NaN above everything, ties to the lower index
- *   stats: aspec_topk_distill_stats_floats() floats per row, for the gradient.
- * A row without a used slot: kl 0, accept 0. Bits of *status_flags (caller-zeroed, may be NULL), with
- * NaN rows: 1 a teacher row out of range, 2 a target out of range, 8 a teacher token out of range, 16
- * a teacher token twice in a row. workspace: of aspec_topk_distill_workspace_bytes (0 for most
+ *   stats: aspec_topk_distill_stats_floats() floats per row, for the gradient (NULL: none follows).
+ * A row without a used slot: kl 0, accept 0. status_words as above: with a NaN row, word 0 is set to 1
+ * for a teacher row out of range, word 1 for a target, word 3 for a teacher token, word 4 for a teacher
+ * token twice in a row. workspace: of aspec_topk_distill_workspace_bytes (0 for most
  * shapes; uninitialised; free once the call's kernels are done).
  *
  * aspec_topk_distill_bwd writes the gradient of sum (grad_ce ce + grad_kl kl) (each may be NULL) in
@@ -433,7 +434,7 @@ int aspec_topk_distill_fwd(const void* logits, int dtype, int64_t rows, int64_t 
                            const float* teacher_logprobs, int64_t kept, const int64_t* teacher_rows,
                            int64_t num_teacher_rows, int renormalize, float temperature, float* ce,
                            float* kl, float* accept, int64_t* argmax, float* stats, void* workspace,
-                           int32_t* status_flags, void* stream);
+                           int32_t* status_words, void* stream);
 int aspec_topk_distill_bwd(const void* logits, int dtype, int64_t rows, int64_t vocab,
                            int64_t row_stride, const int64_t* targets, int64_t ignore_index,
                            const void* teacher_tokens, int token_dtype,
@@ -449,7 +450,7 @@ int aspec_topk_distill_fused_fwd_bwd(const void* logits, int dtype, int64_t rows
                                      int renormalize, float temperature, const float* grad_ce,
                                      const float* grad_kl, float* ce, float* kl, float* accept,
                                      int64_t* argmax, float* stats, void* workspace,
-                                     void* grad_logits, int64_t grad_stride, int32_t* status_flags,
+                                     void* grad_logits, int64_t grad_stride, int32_t* status_words,
                                      void* stream);
 
 /* ---------------------------------------------------------------------------------------------

@@ -135,8 +135,9 @@ def test_refusals_of_the_c_entries():
     refused(NotImplementedError, "128", kept=129)
     for temperature in (0.0, -1.0, float("nan"), float("inf"), 1e-45):
         refused(ValueError, "temperature", temperature=temperature)
-    for bad in ({"logits": None}, {"tokens": None}, {"stats": None}):
+    for bad in ({"logits": None}, {"tokens": None}):
         refused(ValueError, "null pointer", **bad)
+    refused(ValueError, "null pointer", stats=None, which="bwd")
     refused(ValueError, "null pointer", ce=None, which="fwd fused")
     refused(ValueError, "null pointer", grad=None, which="bwd fused")
     refused(ValueError, "null pointer", targets=None, which="bwd fused")  # a gradient of ce without a target
