@@ -114,10 +114,13 @@ __device__ __forceinline__ RowResult finish_row(const FwdArgs& a, int64_t row, c
   return r;
 }
 
+// The given token, and its logit's bits; ignore_index (logit 0 of the row) where there is none. Read
+// by every lane alike, as scalars.
 template <typename E>
-__device__ __forceinline__ float logit_at(const FwdArgs& a, int64_t row, int64_t id) {
-  if (id < 0 || id >= a.V) return 0.f;
-  return E::widen(reinterpret_cast<const typename E::bits*>(a.x)[row * a.stride + id]);
+__device__ __forceinline__ int64_t given_token(const FwdArgs& a, int64_t row, typename E::bits& raw) {
+  const int64_t id = a.ids ? a.ids[row] : a.ignore_index;
+  raw = reinterpret_cast<const typename E::bits*>(a.x)[row * a.stride + (id >= 0 && id < a.V ? id : 0)];
+  return id;
 }
 
 // Block-wide count of what a thread counted; every thread gets it. `scratch` holds one word per wave.
@@ -148,15 +151,12 @@ __global__ __launch_bounds__(T, min_waves(T)) void token_logprobs_kernel(FwdArgs
   const int64_t row = a.parts == 1 ? unit : unit / a.parts;
   const int part = a.parts == 1 ? 0 : static_cast<int>(unit - row * a.parts);
   const auto* x = reinterpret_cast<const typename E::bits*>(a.x) + row * a.stride;
+  typename E::bits raw_id;  // read before the row, so that nothing waits for it at the end
+  const int64_t id = given_token<E>(a, row, raw_id);
   Part<E, T, NV> p;
   p.load(x, RowCut::at<E>(x, a.V), part, a.part_chunks);
-  int64_t id = a.ignore_index;
-  float at_id = 0.f;
-  if (a.parts == 1 && threadIdx.x == 0 && a.ids) {
-    id = a.ids[row];
-    at_id = logit_at<E>(a, row, id);
-  }
 
+  p.arrive();
   // ---- maximum and sums
   float m = kNegInf;
   p.each_value([&](float v) { m = fmaxf(m, v); });
@@ -188,7 +188,7 @@ __global__ __launch_bounds__(T, min_waves(T)) void token_logprobs_kernel(FwdArgs
     if (lane < W) s = Sums{s_m[lane], s_S[lane], s_D[lane]};
     s = merge_wave(s, scale);
     if (a.parts == 1) {
-      r = finish_row(a, row, s, lane == 0, id, at_id);
+      r = finish_row(a, row, s, lane == 0, id, E::widen(raw_id));
       if constexpr (TOP) {
         if (lane == 0) {
           s_row[0] = r.M;
@@ -311,19 +311,15 @@ __global__ __launch_bounds__(kJoinThreads) void token_logprobs_join_kernel(FwdAr
   if (row >= a.rows) return;
   for (int i = threadIdx.x; i < a.parts * K; i += kJoinThreads) s_a[i] = a.part_top[row * a.parts * K + i];
   if (threadIdx.x < 64) {
-    int64_t id = a.ignore_index;
-    float at_id = 0.f;
-    if (lane == 0 && a.ids) {
-      id = a.ids[row];
-      at_id = logit_at<E>(a, row, id);
-    }
+    typename E::bits raw_id;
+    const int64_t id = given_token<E>(a, row, raw_id);
     Sums s{kNegInf, 0.f, 0.f};
     if (lane < a.parts) {
       const float* o = a.part_sums + (row * a.parts + lane) * 3;
       s = Sums{o[0], o[1], o[2]};
     }
     s = merge_wave(s, scale);
-    const RowResult r = finish_row(a, row, s, lane == 0, id, at_id);
+    const RowResult r = finish_row(a, row, s, lane == 0, id, E::widen(raw_id));
     if (lane == 0) {
       s_row[0] = r.M;
       s_row[1] = r.log_s;
@@ -366,11 +362,12 @@ __global__ __launch_bounds__(kJoinThreads) void token_logprobs_join_kernel(FwdAr
 // behind the dense values by the thread that wrote those.
 template <typename E, int T, int NV, bool ENTROPY>
 __global__ __launch_bounds__(T, min_waves(T)) void token_logprobs_bwd_kernel(BwdArgs a) {
+  using P = Part<E, T, NV>;
   __shared__ int s_head[T];
-  __shared__ int s_next[kMaxTop + 1], s_token[kMaxTop + 1];
-  __shared__ float s_g[kMaxTop + 1], s_value[kMaxTop + 1];
+  __shared__ int s_next[kMaxTop], s_token[kMaxTop];
+  __shared__ float s_value[kMaxTop], s_lost;
   const float scale = a.inv_t * kLog2e;
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t unit = unit_of_block();
   if (unit >= a.rows * a.parts) return;
   const int64_t row = a.parts == 1 ? unit : unit / a.parts;
@@ -378,72 +375,78 @@ __global__ __launch_bounds__(T, min_waves(T)) void token_logprobs_bwd_kernel(Bwd
   const auto* x = reinterpret_cast<const typename E::bits*>(a.x) + row * a.stride;
   auto* dx = reinterpret_cast<typename E::bits*>(a.dx) + row * a.dx_stride;
   const RowCut cut = RowCut::at<E>(dx, a.V);
-  Part<E, T, NV> p;
-  p.load(x, cut, part, a.part_chunks);
-  s_head[threadIdx.x] = -1;
-  __syncthreads();
-  // entries 0..K-1: the alternatives; entry K: the given token. Each goes to its thread's chain.
-  for (int k = threadIdx.x; k <= a.K; k += T) {
-    int64_t token = -1;
-    float g = 0.f;
-    if (k < a.K) {
-      if (a.g_top) {
-        token = a.top_indices[row * a.K + k];
-        g = a.g_top[row * a.K + k];
-      }
-    } else if (a.ids && a.g_logprob && a.ids[row] != a.ignore_index) {
-      token = a.ids[row];
-      if (token < 0 || token >= a.V) {  // the forward's check has the error; fails closed here
-        token = -1;
-        g = __builtin_nanf("");
-      } else {
-        g = a.g_logprob[row];
-      }
-    }
-    s_g[k] = g;
-    s_token[k] = static_cast<int>(token);
-    int owner = 0;
-    if (token >= 0 && token < a.V && Part<E, T, NV>::place(cut, part, a.part_chunks, static_cast<int>(token), owner) >= 0)
-      s_next[k] = atomicExch(&s_head[owner], k);
+  // the given token, with its gradient, and the alternatives: read before the row
+  int given = -1;
+  float g_given = 0.f;
+  if (a.ids && a.g_logprob && a.ids[row] != a.ignore_index) {
+    const int64_t id = a.ids[row];
+    if (id >= 0 && id < a.V) given = static_cast<int>(id);
+    g_given = given >= 0 ? a.g_logprob[row] : __builtin_nanf("");  // the forward's check has the error
   }
-  __syncthreads();
-  float G = 0.f;
-  for (int k = lane; k <= a.K; k += 64) G += s_g[k];
-  G = wave_allsum(G);
+  const typename E::bits raw_given = x[max(given, 0)];
   const float4 st = *reinterpret_cast<const float4*>(a.stats + row * kStats);
   const bool empty = st.y == 0.f;  // nothing has a probability, nothing a gradient
   const float base = base_of(st.x), inv_s = empty ? 0.f : 1.f / st.y;
   const float gh = ENTROPY && !empty ? a.g_entropy[row] : 0.f;
+  int64_t token[2];
+  float g[2];
+  const bool top = a.K > 0;
+  if (top && wave == 0) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t at = row * a.K + min(lane + 64 * h, a.K - 1);
+      token[h] = a.top_indices[at];
+      g[h] = a.g_top[at];
+    }
+  }
+  P p;
+  p.load(x, cut, part, a.part_chunks);
+  float lost = g_given;  // G
+  if (top) {
+    s_head[threadIdx.x] = -1;
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = lane + 64 * h;
+        if (k >= a.K) g[h] = 0.f;
+        const int t = k < a.K && token[h] >= 0 && token[h] < a.V ? static_cast<int>(token[h]) : -1;
+        int owner = 0;
+        if (t >= 0 && P::place(cut, part, a.part_chunks, t, owner) >= 0) {
+          s_next[k] = atomicExch(&s_head[owner], k);
+          s_token[k] = t;
+          s_value[k] = g[h];
+        }
+      }
+      lost += wave_allsum(g[0] + g[1]);
+      if (lane == 0) s_lost = lost;
+    }
+    __syncthreads();
+    lost = s_lost;
+  }
   // logp + H = ln2 (d - D / S), so dx = e (u + v d) with e = exp2(d)
   const float v = -gh * kLn2 * inv_s * a.inv_t;
-  const float u = empty ? 0.f : (gh * kLn2 * st.w - G) * inv_s * a.inv_t;
+  const float u = empty ? 0.f : (gh * kLn2 * st.w - lost) * inv_s * a.inv_t;
   const auto dense = [&](float xv) {
     const float d = (xv - base) * scale, e = fast_exp2(d);
     if constexpr (ENTROPY) return e * fmaf(v, fmaxf(d, -200.f), u);
     else return e * u;
   };
-  // the same token may be an alternative and the given one: the alternative's entry writes both
-  const int own = s_head[threadIdx.x];
-  const bool any = own >= 0;
-  if (any) {
-    for (int k = own; k >= 0; k = s_next[k]) {
-      float value = dense(E::widen(x[s_token[k]]));
-      if (!empty) {
-        value += s_g[k] * a.inv_t;
-        if (k < a.K && s_token[a.K] == s_token[k]) value += s_g[a.K] * a.inv_t;
-      }
-      s_value[k] = value;
-    }
-  }
+  const float direct = empty ? 0.f : a.inv_t;  // of a token's own gradient
+  p.arrive();
   p.store(dx, dense);
-  if (any) {
-    for (int k = own; k >= 0; k = s_next[k]) {
-      bool twice = false;
-      if (k == a.K)
-        for (int j = own; j >= 0; j = s_next[j]) twice |= j != k && s_token[j] == s_token[k];
-      if (!twice) dx[s_token[k]] = E::narrow(s_value[k]);
+  // an alternative may be the given token too
+  bool both = false;
+  if (top)
+    for (int k = s_head[threadIdx.x]; k >= 0; k = s_next[k]) {
+      const bool is_given = s_token[k] == given;
+      both |= is_given;
+      dx[s_token[k]] = E::narrow(dense(E::widen(x[s_token[k]])) + (s_value[k] + (is_given ? g_given : 0.f)) * direct);
     }
-  }
+  int owner = -1;
+  if (given >= 0 && P::place(cut, part, a.part_chunks, given, owner) >= 0 && owner == static_cast<int>(threadIdx.x) &&
+      !both)
+    dx[given] = E::narrow(dense(E::widen(raw_given)) + g_given * direct);
 }
 
 template <typename E, int T, int NV>

@@ -76,6 +76,11 @@ struct Args {
   int64_t dx_stride;
 };
 
+struct Target {
+  int token;   // -1: none
+  bool bad;
+};
+
 // The kept tokens of a row in LDS, and their chains: entry k hangs in the chain of the thread that
 // holds its token.
 template <int T>
@@ -85,6 +90,11 @@ struct Kept {
   float x[kMaxTop], lp[kMaxTop], value[kMaxTop + 1];
   double q[kMaxTop];   // exp(lp); 0 for an unused slot
   int poison;          // an index that the row cannot be computed with
+  // A used entry's logit and probability, an unused one's absence.
+  __device__ __forceinline__ void fill(int k, float logit) {
+    x[k] = token[k] >= 0 ? logit : kNegInf;
+    q[k] = token[k] >= 0 ? exp64(lp[k]) : 0.;
+  }
 };
 
 // The teacher's row, or -1.
@@ -94,22 +104,27 @@ __device__ __forceinline__ int64_t teacher_row(const Args& a, int64_t row) {
   return t < 0 || t >= a.trows ? -1 : t;
 }
 
-// Entry k of teacher row t: its token (-1: none) and log-probability; `bad` where it is neither.
-__device__ __forceinline__ int read_entry(const Args& a, int64_t t, int k, float& lp, bool& bad) {
-  if (t < 0) return -1;
-  const int64_t at = t * a.K + k;
-  const int64_t token = a.tokens64 ? reinterpret_cast<const int64_t*>(a.tokens)[at]
-                                   : reinterpret_cast<const int32_t*>(a.tokens)[at];
-  lp = a.logprobs[at];
-  if (token >= 0 && token < a.V) return static_cast<int>(token);
-  bad |= token != -1;
+// Entry k of teacher row t: its token as two words (read alike whatever its type, so that no load
+// waits in a branch) and its log-probability. Places that are not there read entry 0 of row 0.
+struct RawEntry {
+  uint32_t low, high;
+  float lp;
+};
+__device__ __forceinline__ RawEntry load_entry(const Args& a, int64_t t, int k) {
+  const int64_t at = max(t, static_cast<int64_t>(0)) * a.K + (k < a.K ? k : 0);
+  const auto* words = reinterpret_cast<const uint32_t*>(a.tokens) + (a.tokens64 ? 2 * at : at);
+  return RawEntry{words[0], words[a.tokens64], a.logprobs[at]};
+}
+// The token, -1 where there is none; `bad` where it is out of range.
+__device__ __forceinline__ int token_of(const Args& a, int64_t t, int k, const RawEntry& e, bool& bad) {
+  if (t < 0 || k >= a.K) return -1;
+  const int token = static_cast<int>(e.low);
+  const int high = a.tokens64 ? static_cast<int>(e.high) : token >> 31;
+  if (high == 0 && token >= 0 && token < a.V) return token;
+  bad |= token != -1 || high != -1;
   return -1;
 }
 
-struct Target {
-  int token;   // -1: none
-  bool bad;
-};
 __device__ __forceinline__ Target read_target(const Args& a, int64_t row) {
   if (!a.targets) return Target{-1, false};
   const int64_t t = a.targets[row];
@@ -294,39 +309,53 @@ __device__ __forceinline__ void forward_unit(const Args& a, int64_t unit, Kept<T
   auto* dx = reinterpret_cast<typename E::bits*>(a.dx) + row * a.dx_stride;
   const RowCut cut = RowCut::at<E>(GRAD ? static_cast<const void*>(dx) : x, a.V);
 
+  // What the row's end needs is read now, so that no load of its own is waited for there: the teacher's
+  // entries by the first wave (their logits are on the way while the row is reduced), the target and
+  // the weights as scalars.
+  const int64_t trow = teacher_row(a, row);
+  const Target target = read_target(a, row);
+  const typename E::bits raw_target = x[max(target.token, 0)];
+  float g_kl = 0.f, g_ce = 0.f;
+  if constexpr (GRAD) {
+    if (a.g_kl) g_kl = a.g_kl[row];
+    if (a.g_ce) g_ce = a.g_ce[row];
+  }
+  RawEntry entry[2];
+  if (wave == 0) {
+    entry[0] = load_entry(a, trow, lane);
+    entry[1] = load_entry(a, trow, lane + 64);
+  }
+  P p;
+  p.load(x, cut, part, a.part_chunks);
   kept.head[threadIdx.x] = -1;
   if (threadIdx.x == 0) {
     kept.poison = 0;
     s_arg = 0;
   }
-  P p;
-  p.load(x, cut, part, a.part_chunks);
   __syncthreads();
+  typename E::bits raw[2] = {0, 0};
   if (wave == 0) {
-    const int64_t trow = teacher_row(a, row);
     bool bad = false;
-#pragma unroll 1
-    for (int k = lane; k < a.K; k += 64) {
-      float lp = 0.f;
-      const int token = read_entry(a, trow, k, lp, bad);
-      int owner = 0;
-      if (token >= 0 && P::place(cut, part, a.part_chunks, token, owner) >= 0)
-        kept.next[k] = atomicExch(&kept.head[owner], k);
-      kept.token[k] = token;
-      if (a.parts == 1) {
-        kept.lp[k] = lp;
-        kept.q[k] = token >= 0 ? exp64(lp) : 0.;
-        kept.x[k] = token >= 0 ? E::widen(x[token]) : kNegInf;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int k = lane + 64 * h;
+      const int token = token_of(a, trow, k, entry[h], bad);
+      raw[h] = x[max(token, 0)];
+      if (k < a.K) {
+        int owner = 0;
+        if (token >= 0 && P::place(cut, part, a.part_chunks, token, owner) >= 0)
+          kept.next[k] = atomicExch(&kept.head[owner], k);
+        kept.token[k] = token;
+        kept.lp[k] = entry[h].lp;
       }
     }
-    if (trow < 0 || __any(bad)) {
-      if (lane == 0) {
-        kept.poison = 1;
-        report(a.status, trow < 0 ? kBadTeacherRow : kBadTeacherToken);
-      }
+    if ((__any(bad) || trow < 0) && lane == 0) {
+      kept.poison = 1;
+      report(a.status, trow < 0 ? kBadTeacherRow : kBadTeacherToken);
     }
   }
   __syncthreads();
+  p.arrive();
   // ---- the kept tokens leave the registers
   for (int k = kept.head[threadIdx.x]; k >= 0; k = kept.next[k]) {
     int owner;
@@ -388,8 +417,10 @@ __device__ __forceinline__ void forward_unit(const Args& a, int64_t unit, Kept<T
         a.part_arg[unit] = s_arg;
       }
     } else {
-      const Target target = read_target(a, row);
-      const float x_target = target.token >= 0 ? E::widen(x[target.token]) : 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (lane + 64 * h < a.K) kept.fill(lane + 64 * h, E::widen(raw[h]));
+      const float x_target = E::widen(raw_target);
       float st[kStats];
       finish_row<TWO>(a, row, lane, t, kept, target, x_target, st);
       if (a.argmax) {
@@ -405,8 +436,8 @@ __device__ __forceinline__ void forward_unit(const Args& a, int64_t unit, Kept<T
       }
       if constexpr (GRAD) {
         // a bad target's NaN takes the whole row of the gradient
-        const float gc = target.bad ? __builtin_nanf("") : target.token >= 0 && a.g_ce ? a.g_ce[row] : 0.f;
-        const Factors f = factors_of<TWO>(st, a.g_kl ? a.g_kl[row] : 0.f, gc, a.inv_t);
+        const float gc = target.bad ? __builtin_nanf("") : target.token >= 0 ? g_ce : 0.f;
+        const Factors f = factors_of<TWO>(st, g_kl, gc, a.inv_t);
 #pragma unroll 1
         for (int k = lane; k < a.K; k += 64)
           if (kept.token[k] >= 0)
@@ -425,7 +456,6 @@ __device__ __forceinline__ void forward_unit(const Args& a, int64_t unit, Kept<T
     const Factors f = s_factors;
     p.store(dx, [&](float v) { return f.template tail<TWO>(v, scale); });
     // behind the dense values, by the thread that wrote those
-    const Target target = read_target(a, row);
     bool kept_target = false;
     for (int k = kept.head[threadIdx.x]; k >= 0; k = kept.next[k]) {
       dx[kept.token[k]] = E::narrow(kept.value[k]);

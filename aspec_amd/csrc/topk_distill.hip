@@ -38,20 +38,17 @@ __global__ __launch_bounds__(64) void topk_distill_join_kernel(Args a) {
   if (row >= a.rows) return;
   const auto* x = reinterpret_cast<const typename E::bits*>(a.x) + row * a.stride;
   const int64_t trow = teacher_row(a, row);
-  bool bad = trow < 0;  // flagged by the parts
+  const Target target = read_target(a, row);
+  const float x_target = E::widen(x[max(target.token, 0)]);
+  bool bad = trow < 0;  // reported by the parts
   uint64_t best = 0;
   for (int k = lane; k < a.K; k += 64) {
-    float lp = 0.f;
-    const int token = read_entry(a, trow, k, lp, bad);
-    kept.token[k] = token;
-    kept.lp[k] = lp;
-    kept.q[k] = token >= 0 ? exp64(lp) : 0.;
-    const float v = token >= 0 ? E::widen(x[token]) : kNegInf;
-    kept.x[k] = v;
-    if (token >= 0) best = max(best, ranked(order_key(v), token));
+    const RawEntry entry = load_entry(a, trow, k);
+    kept.token[k] = token_of(a, trow, k, entry, bad);
+    kept.lp[k] = entry.lp;
+    kept.fill(k, E::widen(x[max(kept.token[k], 0)]));
+    if (kept.token[k] >= 0) best = max(best, ranked(order_key(kept.x[k]), kept.token[k]));
   }
-  const Target target = read_target(a, row);
-  const float x_target = target.token >= 0 ? E::widen(x[target.token]) : 0.f;
   Tail t{kNegInf, 0.f, 0.f};
   if (lane < a.parts) {
     const float4 s = *reinterpret_cast<const float4*>(a.part_sums + (row * a.parts + lane) * 4);
@@ -71,14 +68,14 @@ __global__ __launch_bounds__(64) void topk_distill_join_kernel(Args a) {
   }
 }
 
-// Gradient from the forward's statistics; grad may be the logits' own buffer (a thread reads its
-// elements, the kept ones among them, before it writes any).
+// Gradient from the forward's statistics; it may go to the logits' own buffer (every element is read
+// before the barrier that the first one is written behind).
 template <typename E, int T, int NV, bool TWO>
 __global__ __launch_bounds__(T, min_waves(T)) void topk_distill_bwd_kernel(Args a) {
   using P = Part<E, T, NV>;
   __shared__ int s_head[T];
   __shared__ int s_next[kMaxTop], s_token[kMaxTop];
-  __shared__ float s_value[kMaxTop + 1];
+  __shared__ float s_value[kMaxTop];
   const float scale = a.inv_t * kLog2e;
   const int64_t unit = unit_of_block();
   if (unit >= a.rows * a.parts) return;
@@ -87,42 +84,54 @@ __global__ __launch_bounds__(T, min_waves(T)) void topk_distill_bwd_kernel(Args 
   const auto* x = reinterpret_cast<const typename E::bits*>(a.x) + row * a.stride;
   auto* dx = reinterpret_cast<typename E::bits*>(a.dx) + row * a.dx_stride;
   const RowCut cut = RowCut::at<E>(dx, a.V);
-  s_head[threadIdx.x] = -1;
-  P p;
-  p.load(x, cut, part, a.part_chunks);
-  __syncthreads();
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t trow = teacher_row(a, row);
-  for (int k = threadIdx.x; k < a.K; k += T) {
-    float lp = 0.f;
-    bool bad = false;  // the forward has made such a row's statistics NaN
-    const int token = read_entry(a, trow, k, lp, bad);
-    int owner = 0;
-    s_token[k] = token;
-    s_value[k] = expf(lp);
-    if (token >= 0 && P::place(cut, part, a.part_chunks, token, owner) >= 0)
-      s_next[k] = atomicExch(&s_head[owner], k);
-  }
   const Target target = read_target(a, row);
-  const float gc = target.bad ? __builtin_nanf("") : target.token >= 0 && a.g_ce ? a.g_ce[row] : 0.f;
+  const typename E::bits raw_target = x[max(target.token, 0)];
   float st[kStats];
 #pragma unroll
   for (int i = 0; i < kStats; ++i) st[i] = a.stats[row * kStats + i];
-  const Factors f = factors_of<TWO>(st, a.g_kl ? a.g_kl[row] : 0.f, gc, a.inv_t);
-  int owner = -1;
-  if (target.token >= 0 && P::place(cut, part, a.part_chunks, target.token, owner) < 0) owner = -1;
-  bool writes_target = owner == static_cast<int>(threadIdx.x);
-  __syncthreads();
-  for (int k = s_head[threadIdx.x]; k >= 0; k = s_next[k]) {
-    const bool is_target = s_token[k] == target.token;
-    s_value[k] = st[1] == 0.f ? 0.f
-                              : f.template kept<TWO>(E::widen(x[s_token[k]]), s_value[k] * f.c, is_target, scale);
-    if (is_target) writes_target = false;
+  const float g_kl = a.g_kl ? a.g_kl[row] : 0.f, g_ce = a.g_ce ? a.g_ce[row] : 0.f;
+  RawEntry entry[2];
+  if (wave == 0) {
+    entry[0] = load_entry(a, trow, lane);
+    entry[1] = load_entry(a, trow, lane + 64);
   }
-  float target_value = 0.f;
-  if (writes_target && st[1] != 0.f) target_value = f.template tail<TWO>(E::widen(x[target.token]), scale) - gc;
+  P p;
+  p.load(x, cut, part, a.part_chunks);
+  s_head[threadIdx.x] = -1;
+  const float gc = target.bad ? __builtin_nanf("") : target.token >= 0 ? g_ce : 0.f;
+  const Factors f = factors_of<TWO>(st, g_kl, gc, a.inv_t);
+  __syncthreads();
+  if (wave == 0) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int k = lane + 64 * h;
+      bool bad = false;  // the forward has made such a row's statistics NaN
+      const int token = token_of(a, trow, k, entry[h], bad);
+      const typename E::bits raw = x[max(token, 0)];
+      int owner = 0;
+      if (token < 0 || P::place(cut, part, a.part_chunks, token, owner) < 0) continue;
+      s_next[k] = atomicExch(&s_head[owner], k);
+      s_token[k] = token;
+      s_value[k] = st[1] == 0.f ? 0.f
+                                : f.template kept<TWO>(E::widen(raw), expf(entry[h].lp) * f.c, token == target.token,
+                                                       scale);
+    }
+  }
+  __syncthreads();
+  p.arrive();
   p.store(dx, [&](float v) { return f.template tail<TWO>(v, scale); });
-  for (int k = s_head[threadIdx.x]; k >= 0; k = s_next[k]) dx[s_token[k]] = E::narrow(s_value[k]);
-  if (writes_target) dx[target.token] = E::narrow(target_value);
+  bool kept_target = false;
+  for (int k = s_head[threadIdx.x]; k >= 0; k = s_next[k]) {
+    dx[s_token[k]] = E::narrow(s_value[k]);
+    kept_target |= s_token[k] == target.token;
+  }
+  int owner = -1;
+  if (target.token >= 0 && P::place(cut, part, a.part_chunks, target.token, owner) >= 0 &&
+      owner == static_cast<int>(threadIdx.x) && !kept_target)
+    dx[target.token] =
+        E::narrow(st[1] == 0.f ? 0.f : f.template tail<TWO>(E::widen(raw_target), scale) - gc);
 }
 
 template <typename E, int T, int NV>

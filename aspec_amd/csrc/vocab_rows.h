@@ -125,27 +125,31 @@ struct Part {
   static constexpr int CH = E::kPerChunk;
   uint4 w[NV];
   float edge;     // -inf where this thread has none
+  typename E::bits edge_raw;
   int edge_at;    // its index in the row, or -1
   int held;       // chunks that this thread has
   int first;      // index in the row of its first chunk; the next ones are T chunks apart each
 
+  // Every load is made, of the row's first chunk where the thread has none: a load in a branch is
+  // waited for at the branch's end, one latency each. arrive() puts -inf there; what is done between
+  // the two does not wait for the row.
   __device__ __forceinline__ void load(const typename E::bits* row, const RowCut& rc, int part, int part_chunks) {
     const int t = threadIdx.x, c0 = part * part_chunks;
-    held = (min(part_chunks, rc.chunks - c0) - t + T - 1) / T;
+    held = max(0, (min(part_chunks, rc.chunks - c0) - t + T - 1) / T);
     first = rc.lead + (c0 + t) * CH;
+    const int behind = rc.lead + rc.chunks * CH + t - CH;
+    edge_at = part != 0 ? -1 : t < rc.lead ? t : t >= CH && behind < rc.V ? behind : -1;
+    edge_raw = row[max(edge_at, 0)];
+    if (rc.chunks > 0) {  // uniform
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      w[v] = all_neg_inf<E>();
-      if (v < held) w[v] = load16<E>(row, first + v * (T * CH));
+      for (int v = 0; v < NV; ++v) w[v] = load16<E>(row, v < held ? first + v * (T * CH) : rc.lead);
     }
-    edge = kNegInf;
-    edge_at = -1;
-    if (part == 0) {
-      const int behind = rc.lead + rc.chunks * CH + t - CH;
-      if (t < rc.lead) edge_at = t;
-      else if (t >= CH && behind < rc.V) edge_at = behind;
-      if (edge_at >= 0) edge = E::widen(row[edge_at]);
-    }
+  }
+  __device__ __forceinline__ void arrive() {
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+      if (v >= held) w[v] = all_neg_inf<E>();
+    edge = edge_at >= 0 ? E::widen(edge_raw) : kNegInf;
   }
 
   // Makes the chunks opaque to the compiler, so that the next pass over them widens them, compares
