@@ -105,6 +105,8 @@ __device__ __forceinline__ void store16(typename E::bits* row, int at, const uin
   store_chunk(reinterpret_cast<uint16_t*>(reinterpret_cast<char*>(row) + off), v);
 }
 
+__device__ const uint4 kNoChunk = {};
+
 // ---- how a row is cut ----------------------------------------------------------------------------
 // `lead` elements, then `chunks` whole chunks, then the rest up to V.
 struct RowCut {
@@ -140,10 +142,11 @@ struct Part {
     const int behind = rc.lead + rc.chunks * CH + t - CH;
     edge_at = part != 0 ? -1 : t < rc.lead ? t : t >= CH && behind < rc.V ? behind : -1;
     edge_raw = row[max(edge_at, 0)];
-    if (rc.chunks > 0) {  // uniform
+    const bool any = rc.chunks > 0;  // a row without a whole chunk reads one that is nobody's
+    const auto* src = any ? row : reinterpret_cast<const typename E::bits*>(&kNoChunk);
+    const int none = any ? rc.lead : 0;
 #pragma unroll
-      for (int v = 0; v < NV; ++v) w[v] = load16<E>(row, v < held ? first + v * (T * CH) : rc.lead);
-    }
+    for (int v = 0; v < NV; ++v) w[v] = load16<E>(src, v < held ? first + v * (T * CH) : none);
   }
   __device__ __forceinline__ void arrive() {
 #pragma unroll
