@@ -16,7 +16,7 @@
 // place is the number of list entries above it. Order is by logit, ties by index: (ordered bits,
 // ~index) as one 64-bit number, no two alike. A list that overflows (long runs of equal logits,
 // large ones that share threads) is replaced by exactly the K best, found by bisection with counts
-// over the registers: first the K-th largest value, then the index up to which its ties belong.
+// over the part: first the K-th largest value, then the index up to which its ties belong.
 #include "vocab_rows.h"
 
 namespace aspec {
@@ -137,9 +137,12 @@ __device__ __forceinline__ uint32_t block_count(uint32_t n, uint32_t* scratch) {
 }
 
 template <typename E, int T, int NV, bool TOP>
-__global__ __launch_bounds__(T, min_waves(T)) void token_logprobs_kernel(FwdArgs a) {
+__global__ __launch_bounds__(T, 8) void token_logprobs_kernel(FwdArgs a) {
+  using P = Part<E, T, NV>;
   constexpr int W = T / 64;
   __shared__ float s_m[W], s_S[W], s_D[W];
+  __shared__ uint16_t s_reach[TOP ? T : 1];  // threads whose maximum reaches the bound
+  __shared__ uint32_t s_reached;
   __shared__ uint32_t s_best[TOP ? T : 1], s_count[W];
   __shared__ uint32_t s_n, s_bound;
   __shared__ float s_row[4];
@@ -153,8 +156,9 @@ __global__ __launch_bounds__(T, min_waves(T)) void token_logprobs_kernel(FwdArgs
   const auto* x = reinterpret_cast<const typename E::bits*>(a.x) + row * a.stride;
   typename E::bits raw_id;  // read before the row, so that nothing waits for it at the end
   const int64_t id = given_token<E>(a, row, raw_id);
-  Part<E, T, NV> p;
-  p.load(x, RowCut::at<E>(x, a.V), part, a.part_chunks);
+  const RowCut cut = RowCut::at<E>(x, a.V);
+  P p;
+  p.load(x, cut, part, a.part_chunks);
 
   p.arrive();
   // ---- maximum and sums
@@ -179,7 +183,7 @@ __global__ __launch_bounds__(T, min_waves(T)) void token_logprobs_kernel(FwdArgs
   if constexpr (TOP) {
     // at most the key of the thread's largest token (the maximum skips a NaN, the highest key)
     s_best[threadIdx.x] = order_key(m);
-    if (threadIdx.x == 0) s_n = 0;
+    if (threadIdx.x == 0) s_n = s_reached = 0;
   }
   __syncthreads();
   RowResult r{0.f, 0.f, 0.f, false};
@@ -232,25 +236,49 @@ __global__ __launch_bounds__(T, min_waves(T)) void token_logprobs_kernel(FwdArgs
       if (lane == 0) s_bound = low;
     }
     __syncthreads();
-    // ---- the list
+    // ---- the list: the chunks of the few threads whose maximum reaches the bound are dealt out to all
+    // threads, which read them again (from L2) and list what reaches it
     const uint32_t bound = s_bound;
     const float bound_value = key_value(bound);  // a NaN bound lists every token
+    const int chunks = P::chunks_in(cut, part, a.part_chunks);
     const auto append = [&](float v, int at) {
       const uint32_t slot = atomicAdd(&s_n, 1u);
-      if (slot < kList) s_list[slot] = ranked(order_key(v), at);
+      if (slot < kList) s_list[slot] = (static_cast<uint64_t>(__float_as_uint(v)) << 32) | static_cast<uint32_t>(at);
     };
-    if (!(m < bound_value) || S != S)
-      p.each([&](float v, int at) {
-        if (!(v < bound_value)) append(v, at);
-      });
+    if (!(m < bound_value) || S != S) s_reach[atomicAdd(&s_reached, 1u)] = static_cast<uint16_t>(threadIdx.x);
+    if (p.edge_at >= 0 && !(p.edge < bound_value)) append(p.edge, p.edge_at);
+    __syncthreads();
+    const int tasks = static_cast<int>(s_reached) * NV;
+    for (int task = threadIdx.x; task < tasks; task += T) {
+      const int c = s_reach[task / NV] + (task % NV) * T;
+      if (c >= chunks) continue;
+      const int first = P::index_of(cut, part, a.part_chunks, c);
+      const uint4 w = load16<E>(x, first);
+      uint32_t hits = 0;
+#pragma unroll
+      for (int i = 0; i < P::CH; ++i) hits |= element<E>(w, i) < bound_value ? 0u : 1u << i;
+      for (; hits; hits &= hits - 1) {
+        const int i = __builtin_ctz(hits);
+        append(element_at<E>(w, i), first + i);
+      }
+    }
     __syncthreads();
     if (s_n > kList) {
       // ---- exactly the K best: their smallest value, then the last index among its ties
       const uint32_t K = a.K;
+      const auto each = [&](auto f) {  // every element of the part, read again
+#pragma unroll 1
+        for (int c = threadIdx.x; c < chunks; c += T) {
+          const int first = P::index_of(cut, part, a.part_chunks, c);
+          const uint4 w = load16<E>(x, first);
+#pragma unroll
+          for (int i = 0; i < P::CH; ++i) f(element<E>(w, i), first + i);
+        }
+        if (p.edge_at >= 0) f(p.edge, p.edge_at);
+      };
       const auto count = [&](auto pred) {
         uint32_t n = 0;
-        p.forget();
-        p.each([&](float v, int at) { n += pred(order_key(v), at) ? 1u : 0u; });
+        each([&](float v, int at) { n += pred(order_key(v), at) ? 1u : 0u; });
         return block_count<T>(n, s_count);
       };
       uint32_t low = bound, high = 0xffffffffu;
@@ -270,7 +298,7 @@ __global__ __launch_bounds__(T, min_waves(T)) void token_logprobs_kernel(FwdArgs
       __syncthreads();
       if (threadIdx.x == 0) s_n = 0;
       __syncthreads();
-      p.each([&](float v, int at) {
+      each([&](float v, int at) {
         const uint32_t k = order_key(v);
         if (k > low || (k == low && at <= last)) append(v, at);
       });
@@ -279,12 +307,20 @@ __global__ __launch_bounds__(T, min_waves(T)) void token_logprobs_kernel(FwdArgs
     // ---- each entry's place; at least K entries, or all of a part that has fewer
     const int n = s_n;
     for (int i = threadIdx.x; i < n; i += T) {
-      const uint64_t mine = s_list[i];
-      int place = 0;
-      for (int j = 0; j < n; ++j) place += s_list[j] > mine ? 1 : 0;
-      if (place >= a.K) continue;
+      const uint64_t e = s_list[i];
+      s_list[i] = ranked(order_key(__uint_as_float(static_cast<uint32_t>(e >> 32))), static_cast<int>(static_cast<uint32_t>(e)));
+    }
+    __syncthreads();
+    const RowResult rr{s_row[0], a.inv_t, s_row[1], s_row[2] != 0.f};
+    for (int base = 0; base < n; base += T / 4) {  // four threads to an entry
+      const int i = base + static_cast<int>(threadIdx.x >> 2);
+      const uint64_t mine = i < n ? s_list[i] : 0;
+      uint32_t place = 0;
+      for (int j = threadIdx.x & 3; j < n; j += 4) place += s_list[j] > mine ? 1u : 0u;
+      place += dpp_u32<0xB1>(place);
+      place += dpp_u32<0x4E>(place);
+      if (i >= n || (threadIdx.x & 3) != 0 || place >= static_cast<uint32_t>(a.K)) continue;
       if (a.parts == 1) {
-        const RowResult rr{s_row[0], a.inv_t, s_row[1], s_row[2] != 0.f};
         a.top_logprobs[row * a.K + place] = rr.logprob(ranked_value(mine));
         a.top_indices[row * a.K + place] = ranked_index(mine);
       } else {
@@ -361,7 +397,7 @@ __global__ __launch_bounds__(kJoinThreads) void token_logprobs_join_kernel(FwdAr
 // Gradient: dense over a part, then the few elements that carry a token of their own, written
 // behind the dense values by the thread that wrote those.
 template <typename E, int T, int NV, bool ENTROPY>
-__global__ __launch_bounds__(T, min_waves(T)) void token_logprobs_bwd_kernel(BwdArgs a) {
+__global__ __launch_bounds__(T, 8) void token_logprobs_bwd_kernel(BwdArgs a) {
   using P = Part<E, T, NV>;
   __shared__ int s_head[T];
   __shared__ int s_next[kMaxTop], s_token[kMaxTop];

@@ -18,7 +18,7 @@ namespace {
 using namespace distill;
 
 template <typename E, int T, int NV, bool TWO>
-__global__ __launch_bounds__(T, min_waves(T)) void topk_distill_kernel(Args a) {
+__global__ __launch_bounds__(T, 8) void topk_distill_kernel(Args a) {
   __shared__ Kept<T> kept;
   __shared__ float s_m[T / 64], s_s[T / 64], s_s1[T / 64];
   __shared__ uint64_t s_arg;
@@ -71,7 +71,7 @@ __global__ __launch_bounds__(64) void topk_distill_join_kernel(Args a) {
 // Gradient from the forward's statistics; it may go to the logits' own buffer (every element is read
 // before the barrier that the first one is written behind).
 template <typename E, int T, int NV, bool TWO>
-__global__ __launch_bounds__(T, min_waves(T)) void topk_distill_bwd_kernel(Args a) {
+__global__ __launch_bounds__(T, 8) void topk_distill_bwd_kernel(Args a) {
   using P = Part<E, T, NV>;
   __shared__ int s_head[T];
   __shared__ int s_next[kMaxTop], s_token[kMaxTop];

@@ -85,6 +85,16 @@ __device__ __forceinline__ float element(const uint4& w, int i) {
   else return E::from_word(word_of(w, i >> 1), i & 1);
 }
 
+// Element i of a chunk, i at run time.
+template <typename E>
+__device__ __forceinline__ float element_at(const uint4& w, int i) {
+  constexpr int per = E::kPerChunk / 4;
+  const int j = i / per;
+  const uint32_t a = j & 1 ? w.y : w.x, b = j & 1 ? w.w : w.z, word = j & 2 ? b : a;
+  if constexpr (per == 1) return __uint_as_float(word);
+  else return E::widen(static_cast<uint16_t>(i & 1 ? word >> 16 : word));
+}
+
 template <typename E>
 __device__ __forceinline__ uint4 all_neg_inf() {
   const uint32_t v = E::kPerChunk == 4 ? E::kNegInfBits : (E::kNegInfBits | (E::kNegInfBits << 16));
@@ -185,6 +195,13 @@ struct Part {
     if (edge_at >= 0) f(edge, edge_at);
   }
 
+  // Chunks of a part, and the row's chunk that is the part's c-th.
+  static __device__ __forceinline__ int chunks_in(const RowCut& rc, int part, int part_chunks) {
+    return max(0, min(part_chunks, rc.chunks - part * part_chunks));
+  }
+  static __device__ __forceinline__ int index_of(const RowCut& rc, int part, int part_chunks, int c) {
+    return rc.lead + (part * part_chunks + c) * CH;
+  }
   // Where a token of the row is held: its place within the thread and, through `owner`, the thread;
   // -1 if another part holds it.
   static __device__ __forceinline__ int place(const RowCut& rc, int part, int part_chunks, int token, int& owner) {
