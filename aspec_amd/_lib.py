@@ -93,6 +93,7 @@ SIGNATURES = {
     ),
     "aspec_topk_distill_stats_floats": (_int, []),
     "aspec_topk_distill_workspace_bytes": (_int, [_int, _i64, _i64, _size_p]),
+    "aspec_topk_distill_reads": (_int, [_int, _i64]),
     "aspec_topk_distill_fwd": (
         _int, [_c_void_p, _int, _i64, _i64, _i64, _c_void_p, _i64, _c_void_p, _int, _c_void_p, _i64, _c_void_p,
                _i64, _int, _f32] + [_c_void_p] * 8

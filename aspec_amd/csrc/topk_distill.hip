@@ -233,6 +233,10 @@ extern "C" int aspec_topk_distill_workspace_bytes(int dtype, int64_t rows, int64
   return ASPEC_OK;
 }
 
+extern "C" int aspec_topk_distill_reads(int dtype, int64_t vocab) {
+  return topk_distill_fused_fits(vocab, per_chunk_of(dtype)) ? 1 : 2;
+}
+
 extern "C" int aspec_topk_distill_fwd(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
                                       const int64_t* targets, int64_t ignore_index, const void* teacher_tokens,
                                       int token_dtype, const float* teacher_logprobs, int64_t kept,

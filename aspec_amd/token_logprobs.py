@@ -28,7 +28,8 @@ from torch.autograd.function import once_differentiable
 from aspec_amd import _lib, _timing
 from aspec_amd._flags import index_flags, on_device, settle
 
-_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+# ASPEC_MASK_* codes of the logits' types
+LOGIT_CODES = {torch.float32: 0, torch.bfloat16: 4, torch.float16: 5}
 
 
 class TokenLogprobs(NamedTuple):
@@ -46,13 +47,13 @@ def logit_rows(logits: torch.Tensor, what: str) -> torch.Tensor:
     adjacent (rows padded to a longer stride among them), else a contiguous copy."""
     if not logits.is_cuda:
         raise ValueError(f"{what} requires CUDA logits")
-    if logits.dtype not in _DTYPES:
+    if logits.dtype not in LOGIT_CODES:
         raise ValueError(f"{what} requires BF16, FP16 or FP32 logits")
     if logits.ndim < 1 or logits.shape[-1] == 0:
         raise ValueError(f"{what} requires logits with a vocabulary dimension")
     vocab = logits.shape[-1]
     rows = logits.numel() // vocab
-    flat = logits.reshape(rows, vocab)
+    flat = logits if logits.ndim == 2 else logits.reshape(rows, vocab)
     if rows and (flat.stride(-1) != 1 and vocab > 1 or flat.stride(0) < vocab and rows > 1):
         flat = flat.contiguous()  # transposed or broadcast rows
     return flat
@@ -60,6 +61,11 @@ def logit_rows(logits: torch.Tensor, what: str) -> torch.Tensor:
 
 def row_stride(flat: torch.Tensor) -> int:
     return flat.stride(0) if flat.shape[0] > 1 else flat.shape[1]
+
+
+def vector(t: torch.Tensor) -> torch.Tensor:
+    """A per-row argument as one contiguous vector."""
+    return t if t.ndim == 1 and t.is_contiguous() else t.reshape(-1).contiguous()
 
 
 def check_temperature(temperature) -> float:
@@ -82,7 +88,7 @@ def _forward(logits, ids, top_k, temperature, ignore_index, check_ids, has_backw
     flat = logit_rows(logits, "token_logprobs")
     rows, vocab = flat.shape
     dev, lead = flat.device, logits.shape[:-1]
-    dtype = _lib.mask_dtype_code(flat)
+    dtype = LOGIT_CODES[flat.dtype]
     work_bytes, stat_floats = _sizes(dtype, rows, vocab, top_k)
     with on_device(dev):
         workspace = torch.empty(work_bytes, dtype=torch.uint8, device=dev) if work_bytes else None
@@ -124,7 +130,7 @@ class _TokenLogprobs(torch.autograd.Function):
         grads = [None if g is None else g.to(torch.float32).contiguous() for g in (g_logprobs, g_entropy, g_top)]
         grad = torch.empty((rows, vocab), dtype=flat.dtype, device=dev)
         with on_device(dev), _timing.region("token_logprobs_bwd"):
-            _lib.call("aspec_token_logprobs_bwd", flat.data_ptr(), _lib.mask_dtype_code(flat), rows, vocab,
+            _lib.call("aspec_token_logprobs_bwd", flat.data_ptr(), LOGIT_CODES[flat.dtype], rows, vocab,
                       row_stride(flat), _lib.ptr(ids), ignore_index, temperature, top_k, _lib.ptr(top_indices),
                       stats.data_ptr(), *map(_lib.ptr, grads), grad.data_ptr(), vocab, _lib.stream_handle(dev))
         # the forward's flag, read with this backward's kernel already queued
@@ -154,7 +160,7 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor | None = None, 
         if token_ids.dtype != torch.int64 or token_ids.device != logits.device or (
                 token_ids.shape != logits.shape[:-1] and token_ids.shape != (rows,)):
             raise ValueError("token_ids must be one int64 token per logit row on the logits device")
-        token_ids = token_ids.reshape(-1).contiguous()
+        token_ids = vector(token_ids)
     args = (logits, token_ids, int(top_k), temperature, int(ignore_index), check_ids)
     if logits.requires_grad and torch.is_grad_enabled():
         return TokenLogprobs(*_TokenLogprobs.apply(*args))

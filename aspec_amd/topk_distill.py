@@ -28,9 +28,10 @@ from torch.autograd.function import once_differentiable
 
 from aspec_amd import _lib, _timing
 from aspec_amd._flags import index_flags, on_device, settle
-from aspec_amd.token_logprobs import check_temperature, logit_rows, row_stride
+from aspec_amd.token_logprobs import LOGIT_CODES, check_temperature, logit_rows, row_stride, vector
 
 _TAILS = {"bucket": 0, "renormalize": 1}
+_TOKEN_CODES = {torch.int64: 1, torch.int32: 2}  # ASPEC_MASK_* codes of the teacher's tokens
 
 
 class _Call:
@@ -48,10 +49,10 @@ class _Call:
         if targets is not None:
             if targets.dtype != torch.int64 or targets.numel() != rows or targets.device != dev:
                 raise ValueError("targets must be one int64 class index per logit row on the logits device")
-            targets = targets.reshape(-1).contiguous()
+            targets = vector(targets)
         if teacher_logprobs.requires_grad:
             raise ValueError("top-logit distillation requires a frozen teacher")
-        if (teacher_indices.dtype not in (torch.int64, torch.int32) or teacher_logprobs.dtype != torch.float32
+        if (teacher_indices.dtype not in _TOKEN_CODES or teacher_logprobs.dtype != torch.float32
                 or teacher_indices.ndim < 1 or teacher_indices.shape != teacher_logprobs.shape
                 or teacher_indices.shape[-1] == 0
                 or teacher_indices.device != dev or teacher_logprobs.device != dev):
@@ -63,29 +64,29 @@ class _Call:
                     or teacher_rows.dtype != torch.int64 or teacher_rows.numel() != rows or teacher_rows.device != dev):
                 raise ValueError("indexed teacher requires a nonempty 2D table and one int64 index per row "
                                  "on the logits device")
-            teacher_rows = teacher_rows.reshape(-1).contiguous()
+            teacher_rows = vector(teacher_rows)
         elif teacher_indices.shape[:-1] != lead and teacher_indices.shape[:-1] != (rows,):
             raise ValueError("a teacher without teacher_rows has one row per logit row")
         self.lead, self.rows, self.kept = lead, rows, kept
         self.targets, self.teacher_rows = targets, teacher_rows
-        self.indices = teacher_indices.reshape(-1, kept).contiguous()
-        self.logprobs = teacher_logprobs.reshape(-1, kept).contiguous()
+        self.indices, self.logprobs = (t if t.ndim == 2 and t.is_contiguous() else t.reshape(-1, kept).contiguous()
+                                       for t in (teacher_indices, teacher_logprobs))
 
     def tensors(self):
         return self.targets, self.indices, self.logprobs, self.teacher_rows
 
     @staticmethod
     def of_logits(flat):
-        return (flat.data_ptr(), _lib.mask_dtype_code(flat), flat.shape[0], flat.shape[1], row_stride(flat))
+        return (flat.data_ptr(), LOGIT_CODES[flat.dtype], flat.shape[0], flat.shape[1], row_stride(flat))
 
     def of_teacher(self):
-        return (_lib.ptr(self.targets), self.ignore_index, self.indices.data_ptr(), _lib.mask_dtype_code(self.indices),
+        return (_lib.ptr(self.targets), self.ignore_index, self.indices.data_ptr(), _TOKEN_CODES[self.indices.dtype],
                 self.logprobs.data_ptr(), self.kept, _lib.ptr(self.teacher_rows), self.indices.shape[0])
 
     def outputs(self, flat, want_argmax, want_stats):
         """(ce, kl, accept_rate, argmax, stats, workspace) to be written; None where not wanted."""
         dev = flat.device
-        work_bytes, stat_floats = _sizes(_lib.mask_dtype_code(flat), *flat.shape)
+        work_bytes, stat_floats = _sizes(LOGIT_CODES[flat.dtype], *flat.shape)
         kl = torch.empty(self.lead, dtype=torch.float32, device=dev)
         return (torch.empty_like(kl) if self.targets is not None else None, kl, torch.empty_like(kl),
                 torch.empty(self.lead, dtype=torch.int64, device=dev) if want_argmax else None,
@@ -99,6 +100,11 @@ def _sizes(dtype: int, rows: int, vocab: int) -> tuple[int, int]:
     lib, size = _lib.load(), ctypes.c_size_t()
     _lib.check(lib.aspec_topk_distill_workspace_bytes(dtype, rows, vocab, ctypes.byref(size)))
     return size.value, lib.aspec_topk_distill_stats_floats()
+
+
+def _read_twice(flat) -> bool:
+    """Whether the one-pass entry makes two passes over such rows, with statistics between them."""
+    return bool(_lib.load().aspec_topk_distill_reads(LOGIT_CODES[flat.dtype], flat.shape[1]) > 1)
 
 
 def _forward(logits, call, want_argmax, check, has_backward):
@@ -197,14 +203,14 @@ def _fused(logits, targets, teacher_indices, teacher_logprobs, ce_weights, kl_we
     for w in (ce_weights, kl_weights):
         if w is not None and (w.numel() != call.rows or w.device != logits.device):
             raise ValueError("objective weights must hold one value per logit row on the logits device")
-        weights.append(None if w is None else w.detach().reshape(-1).to(torch.float32).contiguous())
+        weights.append(None if w is None else vector(w.detach()).to(torch.float32))
     logits = logits.detach()
     flat = logit_rows(logits, "top-logit distillation")
     if in_place and flat.data_ptr() != logits.data_ptr():
         raise ValueError("in_place needs logits whose rows are evenly spaced and their elements adjacent")
     dev = flat.device
     with on_device(dev):
-        ce, kl, accept, amax, stats, workspace = call.outputs(flat, return_argmax, True)
+        ce, kl, accept, amax, stats, workspace = call.outputs(flat, return_argmax, _read_twice(flat))
         grad = flat if in_place else torch.empty(flat.shape, dtype=flat.dtype, device=dev)
         flags = index_flags(check_indices, dev)
         stream = torch.cuda.current_stream(dev)

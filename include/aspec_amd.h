@@ -423,11 +423,13 @@ int aspec_token_logprobs_bwd(const void* logits, int dtype, int64_t rows, int64_
  *
  * aspec_topk_distill_bwd writes the gradient of sum (grad_ce ce + grad_kl kl) (each may be NULL) in
  * the logits' dtype to grad_logits [rows][grad_stride], from the same teacher and the forward's
- * stats. aspec_topk_distill_fused_fwd_bwd is both in one call, the logits read once up to 163840 (fp32:
- * 81920) to a row. grad_logits may be the logits' own buffer, with their row stride.
+ * stats. aspec_topk_distill_fused_fwd_bwd is both in one call. It reads the logits
+ * aspec_topk_distill_reads() times: once up to 163840 (fp32: 81920) to a row, without stats or
+ * workspace, else twice. grad_logits may be the logits' own buffer, with their row stride.
  */
 int aspec_topk_distill_stats_floats(void);
 int aspec_topk_distill_workspace_bytes(int dtype, int64_t rows, int64_t vocab, size_t* bytes);
+int aspec_topk_distill_reads(int dtype, int64_t vocab);
 int aspec_topk_distill_fwd(const void* logits, int dtype, int64_t rows, int64_t vocab,
                            int64_t row_stride, const int64_t* targets, int64_t ignore_index,
                            const void* teacher_tokens, int token_dtype,
