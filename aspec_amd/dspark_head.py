@@ -26,6 +26,7 @@ from torch.autograd.function import once_differentiable
 from . import _timing
 from .loss import ce_l1_from_logits
 from .sampling import DEFAULT_SAMPLING, compiled_l1_from_logits
+from .topk_distill import topk_distill_from_logits
 
 __all__ = [
     "VanillaMarkov",
@@ -186,12 +187,21 @@ def acceptance_statistics(accept_rate: torch.Tensor, eval_mask: torch.Tensor) ->
     return torch.stack((numerators, denominators))
 
 
+def _table_rows(positions, context):
+    """Rows of a flattened [batch, context, ...] teacher table at [batch, ...] context positions."""
+    rows = positions.flatten(1).long()
+    if rows.shape[0] > 1:
+        rows = rows + torch.arange(rows.shape[0], device=rows.device)[:, None] * context
+    return rows.reshape(-1).contiguous()
+
+
 def dspark_prediction_terms(hidden, target_ids, prev_ids, head_weight, aligned_target_hidden,
                             eval_mask, weights, *, markov_head=None, confidence_head=None,
                             confidence_head_with_markov=True, l1_loss_alpha=1.0,
                             confidence_head_alpha=0.0, prediction_start=0, block_size=None,
                             cached_target_logits=None, cached_draft_logits=None,
-                            cached_target_positions=None, loss_cache=None, l1_sampling=None):
+                            cached_target_positions=None, loss_cache=None, l1_sampling=None,
+                            cached_target_topk=None):
     """Additive DSpark head terms for one block slice (aspec/models/dspark.py:553-636):
     (ce_num, l1_num, conf_num, position_loss, position_correct, acceptance_totals).
 
@@ -209,7 +219,17 @@ def dspark_prediction_terms(hidden, target_ids, prev_ids, head_weight, aligned_t
     dspark.py:111-112, 606-609): CE and the argmax still come from the raw logits, the L1 from
     `aspec_amd.sampling.compiled_l1_from_logits`; as in the reference, `loss_cache` then serves
     neither term.
+    `cached_target_topk` = (tokens, log-probabilities) is a teacher of which only the best tokens were
+    kept, as `aspec_amd.token_logprobs.token_logprobs(top_k=...)` writes them: [B, N, K, top] per row,
+    or, with `cached_target_positions`, a [B, context, top] table. The divergence from its kept tokens
+    (`aspec_amd.topk_distill`, the tokens outside as one event) then takes the L1's place in l1_num,
+    and the acceptance is that of the same pass; it excludes `aligned_target_hidden`,
+    `cached_target_logits`, `l1_sampling` and `loss_cache`.
     """
+    if cached_target_topk is not None and not (aligned_target_hidden is None and cached_target_logits is None
+                                               and l1_sampling is None and loss_cache is None):
+        raise ValueError("cached_target_topk is the teacher: it excludes aligned_target_hidden, "
+                         "cached_target_logits, l1_sampling and loss_cache")
     if cached_draft_logits is not None:
         logits = cached_draft_logits
         if markov_head is not None:
@@ -225,11 +245,7 @@ def dspark_prediction_terms(hidden, target_ids, prev_ids, head_weight, aligned_t
         if cached_target_positions is not None:
             if cached_target_logits is None or cached_target_logits.ndim != 3:
                 raise ValueError("cached_target_positions index a [batch, context, vocab] teacher table")
-            batch, context, _ = cached_target_logits.shape
-            positions = cached_target_positions.flatten(1).long()
-            if batch > 1:
-                positions = positions + torch.arange(batch, device=positions.device)[:, None] * context
-            teacher_index = positions.reshape(-1).contiguous()
+            teacher_index = _table_rows(cached_target_positions, cached_target_logits.shape[1])
             teacher = cached_target_logits.detach().reshape(-1, vocab).contiguous()
         else:
             teacher = cached_target_logits if cached_target_logits is not None else F.linear(
@@ -237,9 +253,20 @@ def dspark_prediction_terms(hidden, target_ids, prev_ids, head_weight, aligned_t
             ).view_as(logits)
             teacher = teacher.detach().contiguous().reshape(-1, vocab)
     flat = logits.reshape(-1, vocab).contiguous()
+    kept_accept = None
     sampled = l1_sampling is not None and tuple(map(tuple, l1_sampling)) != (DEFAULT_SAMPLING,
                                                                               DEFAULT_SAMPLING)
-    if sampled and teacher is not None:
+    if cached_target_topk is not None:
+        tokens, logprobs = (t.detach() for t in cached_target_topk)
+        if cached_target_positions is not None:
+            if tokens.ndim != 3:
+                raise ValueError("cached_target_positions index a [batch, context, top] teacher table")
+            teacher_index = _table_rows(cached_target_positions, tokens.shape[1])
+        top = tokens.shape[-1]
+        ce, l1, kept_accept, argmax = topk_distill_from_logits(
+            flat, target_ids.reshape(-1).long().contiguous(), tokens.reshape(-1, top), logprobs.reshape(-1, top),
+            teacher_rows=teacher_index, return_argmax=True)
+    elif sampled and teacher is not None:
         ce, _, argmax = ce_l1_from_logits(flat, target_ids.reshape(-1).long().contiguous(), None,
                                           return_argmax=True)
         l1 = compiled_l1_from_logits(flat, teacher, l1_sampling[0], l1_sampling[1],
@@ -252,11 +279,11 @@ def dspark_prediction_terms(hidden, target_ids, prev_ids, head_weight, aligned_t
     ce_num = (ce * weights).sum()
     l1_num = logits.new_zeros((), dtype=torch.float32)
     accept_rate = None
-    if teacher is not None:
+    if teacher is not None or kept_accept is not None:
         l1 = l1.view_as(weights)
         if l1_loss_alpha > 0:
             l1_num = (l1 * weights).sum()
-        accept_rate = (1.0 - 0.5 * l1).clamp(0.0, 1.0)
+        accept_rate = (1.0 - 0.5 * l1).clamp(0.0, 1.0) if kept_accept is None else kept_accept.view_as(weights)
     conf_num = logits.new_zeros((), dtype=torch.float32)
     if confidence_head is not None and confidence_head_alpha > 0:
         if accept_rate is None:

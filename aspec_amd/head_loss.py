@@ -11,6 +11,9 @@ g == 1). Against the unfused composition (GEMM, loss forward,
 loss backward, dgrad GEMM) this drops the backward's second read of the logits and teacher rows and
 one kernel launch. Vocabularies the fused pass does not cover (V % 8 != 0 or V > 32768) run that
 composition instead, with the same results.
+
+`selective_head_distillation` is the same operator against a teacher of which only the best tokens
+were kept: the KL divergence of `aspec_amd.topk_distill` in the L1's place.
 """
 
 from __future__ import annotations
@@ -19,7 +22,9 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from aspec_amd import _lib, _timing
+from aspec_amd._flags import settle
 from aspec_amd.loss import _ce_l1_fused, ce_l1_from_logits, fused_grad_vocab
+from aspec_amd.topk_distill import _fused as _topk_distill_fused
 
 
 class _SelectiveHeadObjective(torch.autograd.Function):
@@ -99,3 +104,65 @@ def selective_head_objective(hidden, weight, targets, teacher, *, ce_weights, l1
     if return_argmax:
         return objective, ce.detach(), l1.detach(), out[2]
     return objective, ce.detach(), l1.detach()
+
+
+class _SelectiveHeadDistillation(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, weight_t, targets, indices, logprobs, ce_weights, kl_weights, teacher_rows,
+                tail, temperature, ignore_index, want_argmax, teacher_ready, has_backward):
+        with _timing.region("head_gemm_fwd"):
+            logits = torch.matmul(hidden, weight.t())
+        if teacher_ready is not None:
+            torch.cuda.current_stream(hidden.device).wait_event(teacher_ready)
+        (ce, kl, accept, dlogits, amax), ctx.flags = _topk_distill_fused(
+            logits, targets, indices, logprobs, ce_weights, kl_weights, teacher_rows, tail, temperature, ignore_index,
+            want_argmax, True, True)
+        if not has_backward:
+            settle(ctx.flags)
+        objective = torch.dot(kl_weights.float(), kl)
+        if ce is not None:
+            objective = objective + torch.dot(ce_weights.float(), ce)
+        ctx.save_for_backward(dlogits, weight_t)
+        ctx.mark_non_differentiable(*(t for t in (ce, kl, accept, amax) if t is not None))
+        return objective, ce, kl, accept, amax
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_objective, *unused):
+        dlogits, weight_t = ctx.saved_tensors
+        with _timing.region("head_gemm_dgrad"):
+            dh = torch.matmul(dlogits, weight_t.t())
+        if grad_objective is not None:
+            g = grad_objective.detach().reshape(()).to(device=dh.device, dtype=torch.float32)
+            if dh.dtype == torch.bfloat16:
+                _lib.call("aspec_scale_bf16_by_device_scalar", dh.data_ptr(), dh.numel(), g.data_ptr(),
+                          _lib.stream_handle(dh.device))
+            else:
+                dh = (dh.float() * g).to(dh.dtype)
+        # the loss pass's flags, read with the dgrad GEMM already queued behind it
+        settle(ctx.flags)
+        return (dh,) + (None,) * 14
+
+
+def selective_head_distillation(hidden, weight, targets, teacher_indices, teacher_logprobs, *, ce_weights=None,
+                                kl_weights, teacher_rows=None, weight_t=None, tail="bucket", temperature=1.0,
+                                ignore_index=-100, return_argmax=False, teacher_ready=None):
+    """objective = sum_r (ce_weights[r] ce[r] + kl_weights[r] kl[r]) for the logits hidden W^T against a
+    teacher's kept tokens: vocabulary GEMM, one loss pass that writes dlogits over the logits, and
+    dh = g dlogits W in the backward.
+
+    hidden [rows, H] (differentiable), weight W [V, H] (frozen), `weight_t`, `teacher_ready` as for
+    `selective_head_objective`; the teacher, `targets` (or None, with `ce_weights`), `tail`,
+    `temperature` and the losses as for `aspec_amd.topk_distill.topk_distill_from_logits`. Returns
+    (objective, ce, kl, accept_rate[, argmax]); only the objective carries gradient (to `hidden`)."""
+    if hidden.ndim != 2 or weight.ndim != 2 or hidden.shape[1] != weight.shape[1]:
+        raise ValueError("hidden [rows, H] and weight [V, H] must share H")
+    if weight.requires_grad:
+        raise ValueError("the selective head's vocabulary projection is frozen")
+    if weight_t is None:
+        weight_t = weight.t().contiguous()
+    out = _SelectiveHeadDistillation.apply(
+        hidden, weight, weight_t, targets, teacher_indices, teacher_logprobs,
+        None if ce_weights is None else ce_weights.reshape(-1), kl_weights.reshape(-1), teacher_rows, tail, temperature,
+        ignore_index, return_argmax, teacher_ready, torch.is_grad_enabled() and hidden.requires_grad)
+    return out if return_argmax else out[:4]

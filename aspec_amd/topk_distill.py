@@ -75,12 +75,10 @@ class _Call:
     def tensors(self):
         return self.targets, self.indices, self.logprobs, self.teacher_rows
 
-    @staticmethod
-    def of_logits(flat):
-        return (flat.data_ptr(), LOGIT_CODES[flat.dtype], flat.shape[0], flat.shape[1], row_stride(flat))
-
-    def of_teacher(self):
-        return (_lib.ptr(self.targets), self.ignore_index, self.indices.data_ptr(), _TOKEN_CODES[self.indices.dtype],
+    def head(self, flat):
+        """The arguments that every entry begins with."""
+        return (flat.data_ptr(), LOGIT_CODES[flat.dtype], flat.shape[0], flat.shape[1], row_stride(flat),
+                _lib.ptr(self.targets), self.ignore_index, self.indices.data_ptr(), _TOKEN_CODES[self.indices.dtype],
                 self.logprobs.data_ptr(), self.kept, _lib.ptr(self.teacher_rows), self.indices.shape[0])
 
     def outputs(self, flat, want_argmax, want_stats):
@@ -108,28 +106,29 @@ def _read_twice(flat) -> bool:
 
 
 def _forward(logits, call, want_argmax, check, has_backward):
-    """One forward launch: (results, logit rows, statistics, index flags to be settled)."""
+    """One forward launch: (results, logit rows, statistics, the entry's first arguments, index flags to be
+    settled)."""
     flat = logit_rows(logits, "top-logit distillation")
-    dev = flat.device
+    dev, head = flat.device, call.head(flat)
     with on_device(dev):
         *out, stats, workspace = call.outputs(flat, want_argmax, has_backward)
         flags = index_flags(check, dev)
         stream = torch.cuda.current_stream(dev)
         with _timing.region("topk_distill_fwd"):
-            _lib.call("aspec_topk_distill_fwd", *call.of_logits(flat), *call.of_teacher(), call.renormalize,
-                      call.temperature, *map(_lib.ptr, (*out, stats, workspace)),
-                      None if flags is None else flags.ptr, stream.cuda_stream)
+            _lib.call("aspec_topk_distill_fwd", *head, call.renormalize, call.temperature,
+                      *map(_lib.ptr, (*out, stats, workspace)), None if flags is None else flags.ptr,
+                      stream.cuda_stream)
         if flags is not None:
             flags.record(stream)
-    return tuple(out), flat, stats, flags
+    return tuple(out), flat, stats, head, flags
 
 
 class _TopkDistill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, call, want_argmax, check):
-        out, flat, stats, ctx.flags = _forward(logits, call, want_argmax, check, True)
+        out, flat, stats, ctx.head, ctx.flags = _forward(logits, call, want_argmax, check, True)
         ctx.save_for_backward(flat, stats, *call.tensors())
-        ctx.call, ctx.shape = call, logits.shape
+        ctx.temperature, ctx.shape = call.temperature, logits.shape
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(*(t for t in out[2:] if t is not None))
         return out
@@ -137,14 +136,14 @@ class _TopkDistill(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g_ce, g_kl, *_):
-        flat, stats = ctx.saved_tensors[:2]  # unpacking also checks that no input was changed in place
-        call, dev = ctx.call, flat.device
-        grads = [None if g is None else g.to(torch.float32).contiguous() for g in (g_ce, g_kl)]
+        # the tensors behind ctx.head; unpacking also checks that none of them was changed in place
+        flat, stats = ctx.saved_tensors[:2]
+        dev = flat.device
+        grads = [None if g is None else vector(g.to(torch.float32)) for g in (g_ce, g_kl)]
         grad = torch.empty(flat.shape, dtype=flat.dtype, device=dev)
         with on_device(dev), _timing.region("topk_distill_bwd"):
-            _lib.call("aspec_topk_distill_bwd", *call.of_logits(flat), *call.of_teacher(), call.temperature,
-                      stats.data_ptr(), *map(_lib.ptr, grads), grad.data_ptr(), flat.shape[1],
-                      _lib.stream_handle(dev))
+            _lib.call("aspec_topk_distill_bwd", *ctx.head, ctx.temperature, stats.data_ptr(), *map(_lib.ptr, grads),
+                      grad.data_ptr(), flat.shape[1], _lib.stream_handle(dev))
         # the forward's flags, read with this backward's kernel already queued
         settle(ctx.flags)
         return grad.view(ctx.shape), None, None, None
@@ -175,7 +174,7 @@ def topk_distill_from_logits(logits, targets, teacher_indices, teacher_logprobs,
     if logits.requires_grad and torch.is_grad_enabled():
         out = _TopkDistill.apply(logits, call, return_argmax, check_indices)
     else:
-        out, _, _, flags = _forward(logits, call, return_argmax, check_indices, False)
+        out, _, _, _, flags = _forward(logits, call, return_argmax, check_indices, False)
         settle(flags)
     return out if return_argmax else out[:3]
 
@@ -215,10 +214,9 @@ def _fused(logits, targets, teacher_indices, teacher_logprobs, ce_weights, kl_we
         flags = index_flags(check_indices, dev)
         stream = torch.cuda.current_stream(dev)
         with _timing.region("topk_distill_fused"):
-            _lib.call("aspec_topk_distill_fused_fwd_bwd", *call.of_logits(flat), *call.of_teacher(), call.renormalize,
-                      call.temperature, *map(_lib.ptr, weights),
-                      *map(_lib.ptr, (ce, kl, accept, amax, stats, workspace)), grad.data_ptr(), row_stride(grad),
-                      None if flags is None else flags.ptr, stream.cuda_stream)
+            _lib.call("aspec_topk_distill_fused_fwd_bwd", *call.head(flat), call.renormalize, call.temperature,
+                      *map(_lib.ptr, weights), *map(_lib.ptr, (ce, kl, accept, amax, stats, workspace)),
+                      grad.data_ptr(), row_stride(grad), None if flags is None else flags.ptr, stream.cuda_stream)
         if flags is not None:
             flags.record(stream)
     return (ce, kl, accept, logits if in_place else grad.view(logits.shape), amax), flags
