@@ -1,4 +1,8 @@
-"""Index errors of a launch, reported through pinned host memory.
+"""Launches of the library's entries, and their index errors through pinned host memory.
+
+The host's share counts where a call's kernels take ten microseconds: one function makes the call on
+the device's current stream, with the device made current and the region timed only where that is
+asked for.
 
 A kernel that meets an index it cannot compute with writes NaN and sets a word here: a plain store,
 which only a bad index ever makes, so a launch needs no device flag to be cleared before it and
@@ -12,6 +16,8 @@ import contextlib
 from collections import defaultdict, deque
 
 import torch
+
+from aspec_amd import _lib, _timing
 
 # the words, in the order of include/aspec_amd.h
 _MESSAGES = (
@@ -40,12 +46,9 @@ class IndexFlags:
                 self._home.append(slot)
         if self._slot is None:
             words = torch.zeros(len(_MESSAGES), dtype=torch.int32, pin_memory=True)
-            self._slot = (words, words.numpy(), torch.cuda.Event())
-        self._slot[1][:] = 0
-
-    @property
-    def ptr(self) -> int:
-        return self._slot[0].data_ptr()
+            self._slot = (words, words.numpy(), torch.cuda.Event(), words.data_ptr())
+        self._slot[1].fill(0)
+        self.ptr = self._slot[3]
 
     def record(self, stream: torch.cuda.Stream) -> None:
         self._slot[2].record(stream)
@@ -74,6 +77,16 @@ def settle(flags: IndexFlags | None) -> None:
         flags.raise_if_bad()
 
 
-def on_device(device: torch.device):
-    """`device` as the current one, where it is not already."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def launch(region: str, device: torch.device, flags: IndexFlags | None, entry: str, *args) -> None:
+    """`entry(*args, stream)` on the device's current stream; `flags` are recorded behind it."""
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            return launch(region, device, flags, entry, *args)
+    stream = torch.cuda.current_stream(device)
+    if _timing._enabled:
+        with _timing.region(region):
+            _lib.call(entry, *args, stream.cuda_stream)
+    else:
+        _lib.call(entry, *args, stream.cuda_stream)
+    if flags is not None:
+        flags.record(stream)

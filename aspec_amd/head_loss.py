@@ -22,7 +22,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from aspec_amd import _lib, _timing
-from aspec_amd._flags import settle
+from aspec_amd._launch import settle
 from aspec_amd.loss import _ce_l1_fused, ce_l1_from_logits, fused_grad_vocab
 from aspec_amd.topk_distill import _fused as _topk_distill_fused
 

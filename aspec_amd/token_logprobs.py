@@ -25,8 +25,8 @@ from typing import NamedTuple, Optional
 import torch
 from torch.autograd.function import once_differentiable
 
-from aspec_amd import _lib, _timing
-from aspec_amd._flags import index_flags, on_device, settle
+from aspec_amd import _lib
+from aspec_amd._launch import index_flags, launch, settle
 
 # ASPEC_MASK_* codes of the logits' types
 LOGIT_CODES = {torch.float32: 0, torch.bfloat16: 4, torch.float16: 5}
@@ -68,6 +68,13 @@ def vector(t: torch.Tensor) -> torch.Tensor:
     return t if t.ndim == 1 and t.is_contiguous() else t.reshape(-1).contiguous()
 
 
+def float_grad(g: torch.Tensor | None) -> torch.Tensor | None:
+    """An upstream gradient as the kernels read it."""
+    if g is None or (g.dtype == torch.float32 and g.is_contiguous()):
+        return g
+    return g.to(torch.float32).contiguous()
+
+
 def check_temperature(temperature) -> float:
     temperature = float(temperature)
     if not (math.isfinite(temperature) and temperature > 0.0):
@@ -83,29 +90,29 @@ def _sizes(dtype: int, rows: int, vocab: int, top_k: int) -> tuple[int, int]:
     return size.value, lib.aspec_token_logprobs_stats_floats()
 
 
+def _head(flat, ids, ignore_index, temperature, top_k):
+    """The arguments that both entries begin with."""
+    return (flat.data_ptr(), LOGIT_CODES[flat.dtype], flat.shape[0], flat.shape[1], row_stride(flat), _lib.ptr(ids),
+            ignore_index, temperature, top_k)
+
+
 def _forward(logits, ids, top_k, temperature, ignore_index, check_ids, has_backward):
     """One forward launch: (results, logit rows, statistics, index flags to be settled)."""
     flat = logit_rows(logits, "token_logprobs")
     rows, vocab = flat.shape
     dev, lead = flat.device, logits.shape[:-1]
-    dtype = LOGIT_CODES[flat.dtype]
-    work_bytes, stat_floats = _sizes(dtype, rows, vocab, top_k)
-    with on_device(dev):
-        workspace = torch.empty(work_bytes, dtype=torch.uint8, device=dev) if work_bytes else None
-        entropy = torch.empty(lead, dtype=torch.float32, device=dev)
-        logprobs = torch.empty_like(entropy) if ids is not None else None
-        top = torch.empty((*lead, top_k), dtype=torch.float32, device=dev) if top_k else None
-        top_indices = torch.empty((*lead, top_k), dtype=torch.int64, device=dev) if top_k else None
-        stats = torch.empty((rows, stat_floats), dtype=torch.float32, device=dev) if has_backward else None
-        flags = index_flags(check_ids and ids is not None, dev)
-        stream = torch.cuda.current_stream(dev)
-        with _timing.region("token_logprobs_fwd"):
-            _lib.call("aspec_token_logprobs_fwd", flat.data_ptr(), dtype, rows, vocab, row_stride(flat),
-                      _lib.ptr(ids), ignore_index, temperature, top_k, _lib.ptr(logprobs), entropy.data_ptr(),
-                      _lib.ptr(top), _lib.ptr(top_indices), _lib.ptr(stats), _lib.ptr(workspace),
-                      None if flags is None else flags.ptr, stream.cuda_stream)
-        if flags is not None:
-            flags.record(stream)
+    work_bytes, stat_floats = _sizes(LOGIT_CODES[flat.dtype], rows, vocab, top_k)
+    workspace = torch.empty(work_bytes, dtype=torch.uint8, device=dev) if work_bytes else None
+    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
+    logprobs = torch.empty(lead, dtype=torch.float32, device=dev) if ids is not None else None
+    top = torch.empty((*lead, top_k), dtype=torch.float32, device=dev) if top_k else None
+    top_indices = torch.empty((*lead, top_k), dtype=torch.int64, device=dev) if top_k else None
+    stats = torch.empty((rows, stat_floats), dtype=torch.float32, device=dev) if has_backward else None
+    flags = index_flags(check_ids and ids is not None, dev)
+    ptr = _lib.ptr
+    launch("token_logprobs_fwd", dev, flags, "aspec_token_logprobs_fwd",
+           *_head(flat, ids, ignore_index, temperature, top_k), ptr(logprobs), entropy.data_ptr(), ptr(top),
+           ptr(top_indices), ptr(stats), ptr(workspace), None if flags is None else flags.ptr)
     return (logprobs, entropy, top, top_indices), flat, stats, flags
 
 
@@ -114,7 +121,8 @@ class _TokenLogprobs(torch.autograd.Function):
     def forward(ctx, logits, ids, top_k, temperature, ignore_index, check_ids):
         out, flat, stats, ctx.flags = _forward(logits, ids, top_k, temperature, ignore_index, check_ids, True)
         ctx.save_for_backward(flat, ids, out[3], stats)
-        ctx.parameters = (top_k, temperature, ignore_index, logits.shape)
+        ctx.parameters = (ignore_index, temperature, top_k)
+        ctx.shape = logits.shape
         ctx.set_materialize_grads(False)
         if out[3] is not None:
             ctx.mark_non_differentiable(out[3])
@@ -124,18 +132,14 @@ class _TokenLogprobs(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g_logprobs, g_entropy, g_top, _):
         flat, ids, top_indices, stats = ctx.saved_tensors
-        top_k, temperature, ignore_index, shape = ctx.parameters
-        rows, vocab = flat.shape
-        dev = flat.device
-        grads = [None if g is None else g.to(torch.float32).contiguous() for g in (g_logprobs, g_entropy, g_top)]
-        grad = torch.empty((rows, vocab), dtype=flat.dtype, device=dev)
-        with on_device(dev), _timing.region("token_logprobs_bwd"):
-            _lib.call("aspec_token_logprobs_bwd", flat.data_ptr(), LOGIT_CODES[flat.dtype], rows, vocab,
-                      row_stride(flat), _lib.ptr(ids), ignore_index, temperature, top_k, _lib.ptr(top_indices),
-                      stats.data_ptr(), *map(_lib.ptr, grads), grad.data_ptr(), vocab, _lib.stream_handle(dev))
-        # the forward's flag, read with this backward's kernel already queued
+        g_logprobs, g_entropy, g_top = map(float_grad, (g_logprobs, g_entropy, g_top))
+        grad = torch.empty(flat.shape, dtype=flat.dtype, device=flat.device)
+        ptr = _lib.ptr
+        launch("token_logprobs_bwd", flat.device, None, "aspec_token_logprobs_bwd",
+               *_head(flat, ids, *ctx.parameters), ptr(top_indices), stats.data_ptr(), ptr(g_logprobs), ptr(g_entropy), ptr(g_top), grad.data_ptr(), flat.shape[1])
+        # the forward's flags, read with this backward's kernel already queued
         settle(ctx.flags)
-        return grad.view(shape), None, None, None, None, None
+        return grad if grad.shape == ctx.shape else grad.view(ctx.shape), None, None, None, None, None
 
 
 def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor | None = None, *, top_k: int = 0,

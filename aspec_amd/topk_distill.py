@@ -26,9 +26,9 @@ import functools
 import torch
 from torch.autograd.function import once_differentiable
 
-from aspec_amd import _lib, _timing
-from aspec_amd._flags import index_flags, on_device, settle
-from aspec_amd.token_logprobs import LOGIT_CODES, check_temperature, logit_rows, row_stride, vector
+from aspec_amd import _lib
+from aspec_amd._launch import index_flags, launch, settle
+from aspec_amd.token_logprobs import LOGIT_CODES, check_temperature, float_grad, logit_rows, row_stride, vector
 
 _TAILS = {"bucket": 0, "renormalize": 1}
 _TOKEN_CODES = {torch.int64: 1, torch.int32: 2}  # ASPEC_MASK_* codes of the teacher's tokens
@@ -67,7 +67,7 @@ class _Call:
             teacher_rows = vector(teacher_rows)
         elif teacher_indices.shape[:-1] != lead and teacher_indices.shape[:-1] != (rows,):
             raise ValueError("a teacher without teacher_rows has one row per logit row")
-        self.lead, self.rows, self.kept = lead, rows, kept
+        self.lead, self.rows = lead, rows
         self.targets, self.teacher_rows = targets, teacher_rows
         self.indices, self.logprobs = (t if t.ndim == 2 and t.is_contiguous() else t.reshape(-1, kept).contiguous()
                                        for t in (teacher_indices, teacher_logprobs))
@@ -76,18 +76,15 @@ class _Call:
         return self.targets, self.indices, self.logprobs, self.teacher_rows
 
     def head(self, flat):
-        """The arguments that every entry begins with."""
-        return (flat.data_ptr(), LOGIT_CODES[flat.dtype], flat.shape[0], flat.shape[1], row_stride(flat),
-                _lib.ptr(self.targets), self.ignore_index, self.indices.data_ptr(), _TOKEN_CODES[self.indices.dtype],
-                self.logprobs.data_ptr(), self.kept, _lib.ptr(self.teacher_rows), self.indices.shape[0])
+        return _head(flat, self.targets, self.ignore_index, self.indices, self.logprobs, self.teacher_rows)
 
     def outputs(self, flat, want_argmax, want_stats):
         """(ce, kl, accept_rate, argmax, stats, workspace) to be written; None where not wanted."""
-        dev = flat.device
+        dev, lead = flat.device, self.lead
         work_bytes, stat_floats = _sizes(LOGIT_CODES[flat.dtype], *flat.shape)
-        kl = torch.empty(self.lead, dtype=torch.float32, device=dev)
-        return (torch.empty_like(kl) if self.targets is not None else None, kl, torch.empty_like(kl),
-                torch.empty(self.lead, dtype=torch.int64, device=dev) if want_argmax else None,
+        return (torch.empty(lead, dtype=torch.float32, device=dev) if self.targets is not None else None,
+                torch.empty(lead, dtype=torch.float32, device=dev), torch.empty(lead, dtype=torch.float32, device=dev),
+                torch.empty(lead, dtype=torch.int64, device=dev) if want_argmax else None,
                 torch.empty((self.rows, stat_floats), dtype=torch.float32, device=dev) if want_stats else None,
                 torch.empty(work_bytes, dtype=torch.uint8, device=dev) if work_bytes else None)
 
@@ -100,35 +97,36 @@ def _sizes(dtype: int, rows: int, vocab: int) -> tuple[int, int]:
     return size.value, lib.aspec_topk_distill_stats_floats()
 
 
+def _head(flat, targets, ignore_index, indices, logprobs, teacher_rows):
+    """The arguments that every entry begins with."""
+    return (flat.data_ptr(), LOGIT_CODES[flat.dtype], flat.shape[0], flat.shape[1], row_stride(flat), _lib.ptr(targets),
+            ignore_index, indices.data_ptr(), _TOKEN_CODES[indices.dtype], logprobs.data_ptr(), indices.shape[1],
+            _lib.ptr(teacher_rows), indices.shape[0])
+
+
 def _read_twice(flat) -> bool:
     """Whether the one-pass entry makes two passes over such rows, with statistics between them."""
-    return bool(_lib.load().aspec_topk_distill_reads(LOGIT_CODES[flat.dtype], flat.shape[1]) > 1)
+    return _lib.load().aspec_topk_distill_reads(LOGIT_CODES[flat.dtype], flat.shape[1]) > 1
 
 
 def _forward(logits, call, want_argmax, check, has_backward):
-    """One forward launch: (results, logit rows, statistics, the entry's first arguments, index flags to be
-    settled)."""
+    """One forward launch: (results, logit rows, statistics, index flags to be settled)."""
     flat = logit_rows(logits, "top-logit distillation")
-    dev, head = flat.device, call.head(flat)
-    with on_device(dev):
-        *out, stats, workspace = call.outputs(flat, want_argmax, has_backward)
-        flags = index_flags(check, dev)
-        stream = torch.cuda.current_stream(dev)
-        with _timing.region("topk_distill_fwd"):
-            _lib.call("aspec_topk_distill_fwd", *head, call.renormalize, call.temperature,
-                      *map(_lib.ptr, (*out, stats, workspace)), None if flags is None else flags.ptr,
-                      stream.cuda_stream)
-        if flags is not None:
-            flags.record(stream)
-    return tuple(out), flat, stats, head, flags
+    ce, kl, accept, amax, stats, workspace = call.outputs(flat, want_argmax, has_backward)
+    flags = index_flags(check, flat.device)
+    ptr = _lib.ptr
+    launch("topk_distill_fwd", flat.device, flags, "aspec_topk_distill_fwd", *call.head(flat), call.renormalize,
+           call.temperature, ptr(ce), kl.data_ptr(), accept.data_ptr(), ptr(amax), ptr(stats), ptr(workspace),
+           None if flags is None else flags.ptr)
+    return (ce, kl, accept, amax), flat, stats, flags
 
 
 class _TopkDistill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, call, want_argmax, check):
-        out, flat, stats, ctx.head, ctx.flags = _forward(logits, call, want_argmax, check, True)
+        out, flat, stats, ctx.flags = _forward(logits, call, want_argmax, check, True)
         ctx.save_for_backward(flat, stats, *call.tensors())
-        ctx.temperature, ctx.shape = call.temperature, logits.shape
+        ctx.parameters = (call.ignore_index, call.temperature, logits.shape)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(*(t for t in out[2:] if t is not None))
         return out
@@ -136,17 +134,15 @@ class _TopkDistill(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g_ce, g_kl, *_):
-        # the tensors behind ctx.head; unpacking also checks that none of them was changed in place
-        flat, stats = ctx.saved_tensors[:2]
-        dev = flat.device
-        grads = [None if g is None else vector(g.to(torch.float32)) for g in (g_ce, g_kl)]
-        grad = torch.empty(flat.shape, dtype=flat.dtype, device=dev)
-        with on_device(dev), _timing.region("topk_distill_bwd"):
-            _lib.call("aspec_topk_distill_bwd", *ctx.head, ctx.temperature, stats.data_ptr(), *map(_lib.ptr, grads),
-                      grad.data_ptr(), flat.shape[1], _lib.stream_handle(dev))
+        flat, stats, targets, indices, logprobs, teacher_rows = ctx.saved_tensors
+        ignore_index, temperature, shape = ctx.parameters
+        g_ce, g_kl = float_grad(g_ce), float_grad(g_kl)
+        grad = torch.empty(flat.shape, dtype=flat.dtype, device=flat.device)
+        launch("topk_distill_bwd", flat.device, None, "aspec_topk_distill_bwd",
+               *_head(flat, targets, ignore_index, indices, logprobs, teacher_rows), temperature, stats.data_ptr(), _lib.ptr(g_ce), _lib.ptr(g_kl), grad.data_ptr(), flat.shape[1])
         # the forward's flags, read with this backward's kernel already queued
         settle(ctx.flags)
-        return grad.view(ctx.shape), None, None, None
+        return grad if grad.shape == shape else grad.view(shape), None, None, None
 
 
 def topk_distill_from_logits(logits, targets, teacher_indices, teacher_logprobs, *, teacher_rows=None, tail="bucket",
@@ -174,7 +170,7 @@ def topk_distill_from_logits(logits, targets, teacher_indices, teacher_logprobs,
     if logits.requires_grad and torch.is_grad_enabled():
         out = _TopkDistill.apply(logits, call, return_argmax, check_indices)
     else:
-        out, _, _, _, flags = _forward(logits, call, return_argmax, check_indices, False)
+        out, _, _, flags = _forward(logits, call, return_argmax, check_indices, False)
         settle(flags)
     return out if return_argmax else out[:3]
 
@@ -207,16 +203,12 @@ def _fused(logits, targets, teacher_indices, teacher_logprobs, ce_weights, kl_we
     flat = logit_rows(logits, "top-logit distillation")
     if in_place and flat.data_ptr() != logits.data_ptr():
         raise ValueError("in_place needs logits whose rows are evenly spaced and their elements adjacent")
-    dev = flat.device
-    with on_device(dev):
-        ce, kl, accept, amax, stats, workspace = call.outputs(flat, return_argmax, _read_twice(flat))
-        grad = flat if in_place else torch.empty(flat.shape, dtype=flat.dtype, device=dev)
-        flags = index_flags(check_indices, dev)
-        stream = torch.cuda.current_stream(dev)
-        with _timing.region("topk_distill_fused"):
-            _lib.call("aspec_topk_distill_fused_fwd_bwd", *call.head(flat), call.renormalize, call.temperature,
-                      *map(_lib.ptr, weights), *map(_lib.ptr, (ce, kl, accept, amax, stats, workspace)),
-                      grad.data_ptr(), row_stride(grad), None if flags is None else flags.ptr, stream.cuda_stream)
-        if flags is not None:
-            flags.record(stream)
+    ce, kl, accept, amax, stats, workspace = call.outputs(flat, return_argmax, _read_twice(flat))
+    grad = flat if in_place else torch.empty(flat.shape, dtype=flat.dtype, device=flat.device)
+    flags = index_flags(check_indices, flat.device)
+    ptr = _lib.ptr
+    launch("topk_distill_fused", flat.device, flags, "aspec_topk_distill_fused_fwd_bwd", *call.head(flat),
+           call.renormalize, call.temperature, ptr(weights[0]), ptr(weights[1]), ptr(ce), kl.data_ptr(),
+           accept.data_ptr(), ptr(amax), ptr(stats), ptr(workspace), grad.data_ptr(), row_stride(grad),
+           None if flags is None else flags.ptr)
     return (ce, kl, accept, logits if in_place else grad.view(logits.shape), amax), flags

@@ -310,3 +310,25 @@ def test_neighbours_stay_as_they_were(gpu):
     out = token_logprobs(buffer[:, :vocab], torch.zeros(7, dtype=torch.int64, device=gpu), top_k=20)
     assert out.logprobs.isfinite().all() and int(out.top_indices.max()) < vocab
     assert buffer[:, vocab:].isnan().all() and torch.equal(buffer[:, :vocab], x)
+
+
+def test_saved_tensors_that_move(gpu):
+    """Saved tensors kept on the host between forward and backward, and logits changed in between."""
+    x, g = logits(gpu, 6, 3000, torch.bfloat16, 97)
+    ids = torch.randint(0, 3000, (6,), device=gpu, generator=g)
+
+    def grad():
+        leaf = x.clone().requires_grad_()
+        out = token_logprobs(leaf, ids, top_k=4)
+        torch.empty(64, 3000, device=gpu).fill_(9)
+        return torch.autograd.grad(out.logprobs.sum() + out.top_logprobs.sum(), leaf)[0]
+
+    want = grad()
+    with torch.autograd.graph.save_on_cpu():
+        assert torch.equal(grad(), want)
+    leaf = x.clone().requires_grad_()
+    twice = leaf * 2
+    out = token_logprobs(twice, ids)
+    twice.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.logprobs.sum().backward()

@@ -390,3 +390,24 @@ def test_teacher_of_token_logprobs(gpu):
                                          cache.top_logprobs[order].flip(-1), teacher_rows=back, temperature=temperature)
         want = topk_distill_from_logits(teacher, None, cache.top_indices, cache.top_logprobs, temperature=temperature)
         torch.testing.assert_close(again[1], want[1], atol=6 * STEPS, rtol=0)
+
+
+def test_saved_tensors_that_move(gpu):
+    """Saved tensors kept on the host between forward and backward, logits or a teacher changed in between."""
+    case = Case(gpu, 6, 3000, 9, torch.bfloat16, 97, table=4)
+    more = {"teacher_rows": case.rows}
+
+    def grad():
+        leaf = case.x.clone().requires_grad_()
+        ce, kl, _ = topk_distill_from_logits(leaf, case.targets, case.tokens, case.logprobs, **more)
+        torch.empty(64, 3000, device=gpu).fill_(9)
+        return torch.autograd.grad([ce, kl], leaf, [case.g_ce, case.g_kl])[0]
+
+    want = grad()
+    with torch.autograd.graph.save_on_cpu():
+        assert torch.equal(grad(), want)
+    leaf = case.x.clone().requires_grad_()
+    _, kl, _ = topk_distill_from_logits(leaf, case.targets, case.tokens, case.logprobs, **more)
+    case.logprobs.sub_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        kl.sum().backward()
