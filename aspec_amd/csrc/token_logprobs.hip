@@ -162,8 +162,7 @@ __global__ __launch_bounds__(T, 8) void token_logprobs_kernel(FwdArgs a) {
 
   p.arrive();
   // ---- maximum and sums
-  float m = kNegInf;
-  p.each_value([&](float v) { m = fmaxf(m, v); });
+  const float m = p.largest();
   const float wm = wave_allmax(m), base = base_of(wm);
   p.forget();
   float S = 0.f, D = 0.f;
@@ -335,25 +334,26 @@ __global__ __launch_bounds__(T, 8) void token_logprobs_kernel(FwdArgs a) {
 // Joins the parts of long rows: the sums by one wave, the ordered lists pairwise. An entry's place
 // in a pair's merged list is its own place plus the number of the other list's entries above it (a
 // binary search); entries past K are dropped.
-constexpr int kJoinThreads = 256;
-template <typename E>
-__global__ __launch_bounds__(kJoinThreads) void token_logprobs_join_kernel(FwdArgs a) {
-  __shared__ uint64_t s_a[kMaxParts * kMaxTop], s_b[kMaxParts * kMaxTop / 2];
+// The lists take parts * K * 12 bytes of LDS (48 KB at most), and a wave does where they are short, so
+// that many rows fit a CU: 1536 rows of ten lists of 8 take 10 us so, 14 with LDS for the longest.
+template <typename E, int T>
+__global__ __launch_bounds__(T) void token_logprobs_join_kernel(FwdArgs a) {
+  extern __shared__ uint64_t s_lists[];
+  uint64_t *const s_a = s_lists, *const s_b = s_lists + a.parts * a.K;
   __shared__ float s_row[4];
   const int lane = threadIdx.x & 63;
   const float scale = a.inv_t * kLog2e;
   const int K = a.K;
   const int64_t row = unit_of_block();
   if (row >= a.rows) return;
-  for (int i = threadIdx.x; i < a.parts * K; i += kJoinThreads) s_a[i] = a.part_top[row * a.parts * K + i];
+  // all the reads before the first wait
+  typename E::bits raw_id;
+  const int64_t id = given_token<E>(a, row, raw_id);
+  const float* o = a.part_sums + (row * a.parts + min(lane, a.parts - 1)) * 3;
+  Sums s{o[0], o[1], o[2]};
+  for (int i = threadIdx.x; i < a.parts * K; i += T) s_a[i] = a.part_top[row * a.parts * K + i];
   if (threadIdx.x < 64) {
-    typename E::bits raw_id;
-    const int64_t id = given_token<E>(a, row, raw_id);
-    Sums s{kNegInf, 0.f, 0.f};
-    if (lane < a.parts) {
-      const float* o = a.part_sums + (row * a.parts + lane) * 3;
-      s = Sums{o[0], o[1], o[2]};
-    }
+    if (lane >= a.parts) s = Sums{kNegInf, 0.f, 0.f};
     s = merge_wave(s, scale);
     const RowResult r = finish_row(a, row, s, lane == 0, id, E::widen(raw_id));
     if (lane == 0) {
@@ -365,7 +365,7 @@ __global__ __launch_bounds__(kJoinThreads) void token_logprobs_join_kernel(FwdAr
   __syncthreads();
   uint64_t *from = s_a, *to = s_b;
   for (int lists = a.parts; lists > 1; lists = (lists + 1) / 2) {
-    for (int i = threadIdx.x; i < lists * K; i += kJoinThreads) {
+    for (int i = threadIdx.x; i < lists * K; i += T) {
       const int list = i / K, at = i - list * K, other = list ^ 1;
       const uint64_t mine = from[i];
       int place = at;
@@ -388,7 +388,7 @@ __global__ __launch_bounds__(kJoinThreads) void token_logprobs_join_kernel(FwdAr
     to = t;
   }
   const RowResult r{s_row[0], a.inv_t, s_row[1], s_row[2] != 0.f};
-  for (int i = threadIdx.x; i < K; i += kJoinThreads) {
+  for (int i = threadIdx.x; i < K; i += T) {
     a.top_logprobs[row * K + i] = r.logprob(ranked_value(from[i]));
     a.top_indices[row * K + i] = ranked_index(from[i]);
   }
@@ -490,7 +490,11 @@ void launch_fwd(const FwdArgs& a, hipStream_t stream) {
   const dim3 grid = grid_of(a.rows * a.parts);
   if (a.K) token_logprobs_kernel<E, T, NV, true><<<grid, T, 0, stream>>>(a);
   else token_logprobs_kernel<E, T, NV, false><<<grid, T, 0, stream>>>(a);
-  if (a.parts > 1) token_logprobs_join_kernel<E><<<grid_of(a.rows), kJoinThreads, 0, stream>>>(a);
+  if (a.parts == 1) return;
+  const unsigned entries = static_cast<unsigned>(a.parts * a.K);
+  const unsigned lds = 8 * (entries + (a.parts + 1) / 2 * a.K);
+  if (entries <= 128) token_logprobs_join_kernel<E, 64><<<grid_of(a.rows), 64, lds, stream>>>(a);
+  else token_logprobs_join_kernel<E, 256><<<grid_of(a.rows), 256, lds, stream>>>(a);
 }
 
 template <typename E, int T, int NV>

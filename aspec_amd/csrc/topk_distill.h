@@ -367,8 +367,7 @@ __device__ __forceinline__ void forward_unit(const Args& a, int64_t unit, Kept<T
       }
   }
   // ---- the tail's maximum and sums
-  float m = kNegInf;
-  p.each_value([&](float v) { m = fmaxf(m, v); });
+  const float m = p.largest();
   const float wm = wave_allmax(m), wbase = base_of(wm);
   p.forget();
   float S = 0.f, S1 = 0.f;

@@ -174,6 +174,37 @@ struct Part {
     asm volatile("" : "+v"(held), "+v"(first));
   }
 
+  // The thread's largest element; a NaN is skipped, or is the result. Sixteen-bit floats are compared
+  // as whole numbers, two to an instruction and without widening: where any is positive, the largest
+  // number is the largest float; where none is, the smallest number is.
+  __device__ __forceinline__ float largest() const {
+    if constexpr (CH == 4) {
+      float m = edge;
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int i = 0; i < CH; ++i) m = fmaxf(m, element<E>(w[v], i));
+      return m;
+    } else {
+      typedef __attribute__((ext_vector_type(2))) short pair;
+      const auto fold = [&](auto op) {
+        pair r = __builtin_bit_cast(pair, w[0].x);
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) r = op(r, __builtin_bit_cast(pair, word_of(w[v], j)));
+        return r;
+      };
+      const pair high = fold([](pair a, pair b) { return __builtin_elementwise_max(a, b); });
+      short best = high.x > high.y ? high.x : high.y;
+      if (best < 0) {
+        const pair low = fold([](pair a, pair b) { return __builtin_elementwise_min(a, b); });
+        best = low.x < low.y ? low.x : low.y;
+      }
+      return fmaxf(E::widen(static_cast<uint16_t>(best)), edge);
+    }
+  }
+
   // f(value) of every element that the thread holds; -inf for the places it does not fill.
   template <typename F>
   __device__ __forceinline__ void each_value(F f) const {
