@@ -15,8 +15,8 @@
 // over the maxima's ordered bits; the tokens at or above it go to a list in LDS, and each one's
 // place is the number of list entries above it. Order is by logit, ties by index: (ordered bits,
 // ~index) as one 64-bit number, no two alike. A list that overflows (long runs of equal logits,
-// large ones that share threads) is replaced by exactly the K best, found by bisection with counts
-// over the part: first the K-th largest value, then the index up to which its ties belong.
+// large ones that share threads) is replaced by exactly the K best: the K-th largest value, found by
+// bisection with counts over the part, and its ties in order.
 #include "vocab_rows.h"
 
 namespace aspec {
@@ -136,6 +136,32 @@ __device__ __forceinline__ uint32_t block_count(uint32_t n, uint32_t* scratch) {
   return sum;
 }
 
+// Of what the threads counted: how much the lower lanes of the wave did.
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t n) {
+  const int lane = threadIdx.x & 63;
+  uint32_t sum = n;
+#pragma unroll
+  for (int off = 1; off < 64; off *= 2) {
+    const uint32_t lower = __shfl_up(sum, off);
+    if (lane >= off) sum += lower;
+  }
+  return sum - n;
+}
+// Adds what the lower waves counted, and returns the block's count; `scratch` holds a word per wave.
+template <int T>
+__device__ __forceinline__ uint32_t block_prefix(uint32_t& before, uint32_t n, uint32_t* scratch) {
+  const int wave = threadIdx.x >> 6;
+  __syncthreads();  // the last count has been read
+  if ((threadIdx.x & 63) == 63) scratch[wave] = before + n;
+  __syncthreads();
+  uint32_t all = 0;
+  for (int w = 0; w < T / 64; ++w) {
+    if (w < wave) before += scratch[w];
+    all += scratch[w];
+  }
+  return all;
+}
+
 template <typename E, int T, int NV, bool TOP>
 __global__ __launch_bounds__(T, 8) void token_logprobs_kernel(FwdArgs a) {
   using P = Part<E, T, NV>;
@@ -144,7 +170,7 @@ __global__ __launch_bounds__(T, 8) void token_logprobs_kernel(FwdArgs a) {
   __shared__ uint16_t s_reach[TOP ? T : 1];  // threads whose maximum reaches the bound
   __shared__ uint32_t s_reached;
   __shared__ uint32_t s_best[TOP ? T : 1], s_count[W];
-  __shared__ uint32_t s_n, s_bound;
+  __shared__ uint32_t s_n, s_bound, s_high;
   __shared__ float s_row[4];
   __shared__ __attribute__((aligned(16))) uint64_t s_list[TOP ? kList : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -219,7 +245,8 @@ __global__ __launch_bounds__(T, 8) void token_logprobs_kernel(FwdArgs a) {
       low = wave_allmin(low);
       high = wave_allmax_u32(high);
       if (a.K > T) low = high = 0;  // fewer maxima than tokens wanted: every token is listed
-      const uint32_t enough = a.K + a.K / 8;
+      if (lane == 0) s_high = high;
+      const uint32_t enough = a.K + a.K / 8 + 4;
       while (low < high) {  // count(>= low) >= K throughout
         const uint32_t mid = low + (high - low) / 2 + ((high - low) & 1);
         uint32_t n = 0;
@@ -249,6 +276,7 @@ __global__ __launch_bounds__(T, 8) void token_logprobs_kernel(FwdArgs a) {
     __syncthreads();
     const int tasks = static_cast<int>(s_reached) * NV;
     for (int task = threadIdx.x; task < tasks; task += T) {
+      if (*static_cast<volatile uint32_t*>(&s_n) > kList) break;  // the list is lost already
       const int c = s_reach[task / NV] + (task % NV) * T;
       if (c >= chunks) continue;
       const int first = P::index_of(cut, part, a.part_chunks, c);
@@ -263,44 +291,76 @@ __global__ __launch_bounds__(T, 8) void token_logprobs_kernel(FwdArgs a) {
     }
     __syncthreads();
     if (s_n > kList) {
-      // ---- exactly the K best: their smallest value, then the last index among its ties
+      // ---- exactly the K best: the K-th largest value by bisection, with counts over the part, which
+      // is read again (from L2) for each; then its ties in the order of their indices
+      constexpr int kDrop = E::kKeyDrop;
       const uint32_t K = a.K;
-      const auto each = [&](auto f) {  // every element of the part, read again
-#pragma unroll 1
-        for (int c = threadIdx.x; c < chunks; c += T) {
-          const int first = P::index_of(cut, part, a.part_chunks, c);
-          const uint4 w = load16<E>(x, first);
+      const auto key = [](float v) { return order_key(v) >> kDrop; };
+      const auto hits = [&](uint4 w, auto pred) {  // one bit for each element of a chunk
+        uint32_t h = 0;
 #pragma unroll
-          for (int i = 0; i < P::CH; ++i) f(element<E>(w, i), first + i);
-        }
-        if (p.edge_at >= 0) f(p.edge, p.edge_at);
+        for (int i = 0; i < P::CH; ++i) h |= pred(key(element<E>(w, i))) ? 1u << i : 0u;
+        return h;
       };
       const auto count = [&](auto pred) {
-        uint32_t n = 0;
-        each([&](float v, int at) { n += pred(order_key(v), at) ? 1u : 0u; });
+        uint32_t n = p.edge_at >= 0 && pred(key(p.edge)) ? 1 : 0;
+#pragma unroll 1
+        for (int c = threadIdx.x; c < chunks; c += T)
+          n += __popc(hits(load16<E>(x, P::index_of(cut, part, a.part_chunks, c)), pred));
         return block_count<T>(n, s_count);
       };
-      uint32_t low = bound, high = 0xffffffffu;
-      if (count([&](uint32_t k, int) { return k > low; }) < K) high = low;
-      while (low < high) {
-        const uint32_t mid = low + (high - low) / 2 + ((high - low) & 1);
-        if (count([&](uint32_t k, int) { return k >= mid; }) >= K) low = mid;
-        else high = mid - 1;
+      uint32_t low = bound >> kDrop, high = s_high >> kDrop;  // count(>= low) >= K throughout
+      uint32_t larger_ones = count([&](uint32_t k) { return k > low; });
+      if (larger_ones >= K) {
+        if (count([&](uint32_t k) { return k > high; }) >= K) {  // NaN, which the maxima skip
+          low = high;
+          high = 0xffffffffu >> kDrop;
+        }
+        while (low < high) {
+          const uint32_t mid = low + (high - low) / 2 + ((high - low) & 1);
+          if (count([&](uint32_t k) { return k >= mid; }) >= K) low = mid;
+          else high = mid - 1;
+        }
+        larger_ones = count([&](uint32_t k) { return k > low; });
       }
-      const uint32_t above = count([&](uint32_t k, int) { return k > low; });
-      int first = 0, last = a.V - 1;
-      while (first < last) {
-        const int mid = first + (last - first) / 2;
-        if (above + count([&](uint32_t k, int at) { return k == low && at <= mid; }) >= K) last = mid;
-        else first = mid + 1;
-      }
+      const auto above = [&](uint32_t k) { return k > low; };
+      const auto tie = [&](uint32_t k) { return k == low; };
+      const uint32_t ties = K - larger_ones;
+      uint32_t seen = 0;
       __syncthreads();
       if (threadIdx.x == 0) s_n = 0;
       __syncthreads();
-      each([&](float v, int at) {
-        const uint32_t k = order_key(v);
-        if (k > low || (k == low && at <= last)) append(v, at);
-      });
+      // Everything above; of the ties the first ones: the edge before the chunks, then T chunks at a
+      // time, then the edge behind them, each thread knowing the number of ties before its own.
+      const auto ties_before = [&](uint32_t tied) {  // and `seen` moves past these threads
+        uint32_t before = wave_prefix(tied);
+        const uint32_t all = block_prefix<T>(before, tied, s_count);
+        before += seen;
+        seen += all;
+        return before;
+      };
+      const bool edge = p.edge_at >= 0, in_front = edge && p.edge_at < cut.lead;
+      const bool edge_tie = edge && tie(key(p.edge));
+      if (edge && above(key(p.edge))) append(p.edge, p.edge_at);
+      if (ties_before(in_front && edge_tie ? 1 : 0) < ties && in_front && edge_tie) append(p.edge, p.edge_at);
+#pragma unroll 1
+      for (int c0 = 0; c0 < chunks; c0 += T) {
+        const int c = c0 + static_cast<int>(threadIdx.x), first = P::index_of(cut, part, a.part_chunks, c);
+        uint4 w = {};
+        uint32_t larger = 0, tied = 0;
+        if (c < chunks) {
+          w = load16<E>(x, first);
+          larger = hits(w, above);
+          tied = hits(w, tie);
+        }
+        const uint32_t before = ties_before(__popc(tied));
+        for (uint32_t left = larger | tied; left; left &= left - 1) {
+          const int i = __builtin_ctz(left);
+          const bool is_tie = (tied >> i) & 1;
+          if (!is_tie || before + __popc(tied & ((1u << i) - 1)) < ties) append(element_at<E>(w, i), first + i);
+        }
+      }
+      if (ties_before(!in_front && edge_tie ? 1 : 0) < ties && !in_front && edge_tie) append(p.edge, p.edge_at);
       __syncthreads();
     }
     // ---- each entry's place; at least K entries, or all of a part that has fewer

@@ -30,6 +30,7 @@ template <typename E>
 void launch_type(const Args& a, bool two, hipStream_t stream) {
   if (a.part_chunks <= 64 * 4) launch<E, 64, 4>(a, two, stream);
   else if (a.part_chunks <= 256 * 4) launch<E, 256, 4>(a, two, stream);
+  else if (a.part_chunks <= 512 * 4) launch<E, 512, 4>(a, two, stream);
   else if (a.part_chunks <= 512 * 8) launch<E, 512, 8>(a, two, stream);
   else if (a.part_chunks <= 1024 * 10) launch<E, 1024, 10>(a, two, stream);
   else launch<E, 1024, 20>(a, two, stream);

@@ -35,6 +35,7 @@ __device__ __forceinline__ void report(int32_t* words, Status s) {
 struct Bf16 {
   using bits = uint16_t;
   static constexpr int kPerChunk = 8;
+  static constexpr int kKeyDrop = 16;  // low bits that no two order_key()s differ in alone
   static constexpr uint32_t kNegInfBits = 0xff80u;
   static __device__ __forceinline__ float widen(uint16_t b) { return bf16_to_f32(b); }
   static __device__ __forceinline__ uint16_t narrow(float f) { return f32_to_bf16_bits(f); }
@@ -46,6 +47,7 @@ struct Bf16 {
 struct F16 {
   using bits = uint16_t;
   static constexpr int kPerChunk = 8;
+  static constexpr int kKeyDrop = 13;  // low bits that no two order_key()s differ in alone
   static constexpr uint32_t kNegInfBits = 0xfc00u;
   static __device__ __forceinline__ float widen(uint16_t b) {
     return static_cast<float>(__builtin_bit_cast(_Float16, b));
@@ -63,6 +65,7 @@ struct F16 {
 struct F32 {
   using bits = uint32_t;
   static constexpr int kPerChunk = 4;
+  static constexpr int kKeyDrop = 0;  // low bits that no two order_key()s differ in alone
   static constexpr uint32_t kNegInfBits = 0xff800000u;
   static __device__ __forceinline__ float widen(uint32_t b) { return __uint_as_float(b); }
   static __device__ __forceinline__ uint32_t narrow(float f) { return __float_as_uint(f); }
@@ -342,16 +345,21 @@ constexpr int64_t kMaxVocab = int64_t{1} << 19;  // 32 parts of 4096 chunks of f
 
 inline int per_chunk_of(int dtype) { return dtype == ASPEC_MASK_F32 ? 4 : 8; }
 
-// Rows of up to 256 chunks take a wave each. Longer rows take workgroups of 512 threads x 8 chunks
-// where that makes two of them for each of the 256 CUs, and 256 x 4 otherwise: with few rows the
-// time is one workgroup's, and four times as many share a row.
+// Rows of up to 256 chunks take a wave each, up to 1024 a workgroup of 256 threads. Longer rows take
+// workgroups of 512 threads where that makes two of them for each of the 256 CUs, and 256 x 4 chunks
+// otherwise: with few rows the time is one workgroup's, and four times as many share a row. The 512
+// hold 8 chunks each, or 4 where that leaves a tenth fewer places empty: 16384 x 4096 logits of 16 bits
+// took 143 us with 512 x 8 (one chunk to a thread, seven places empty), 44 with 256 x 4; 4096 x 16384
+// took 39 with 512 x 8 and take 25 with 512 x 4.
 inline Shape shape_of(int64_t rows, int64_t V, int per_chunk) {
   const int64_t chunks = V / per_chunk;
+  const auto parts = [chunks](int64_t places) { return (chunks + places - 1) / places; };
   Shape s{64, 4, 1, 0};
   if (chunks > 64 * 4) {
-    const int64_t large = (chunks + 4095) / 4096, small = (chunks + 1023) / 1024;
-    const bool many = rows * large >= 512 || small > kMaxParts;
-    s = many ? Shape{512, 8, large, 0} : Shape{256, 4, small, 0};
+    const int64_t few = parts(256 * 4), half = parts(512 * 4), full = parts(512 * 8);
+    if (few == 1 || (rows * full < 512 && few <= kMaxParts)) s = Shape{256, 4, few, 0};
+    else if (half <= kMaxParts && 10 * half * 4 < 9 * full * 8) s = Shape{512, 4, half, 0};
+    else s = Shape{512, 8, full, 0};
   }
   s.part_chunks = (chunks + s.parts - 1) / s.parts;
   return s;
@@ -377,6 +385,7 @@ template <typename E, typename F>
 void dispatch_shape(const Shape& s, F f) {
   if (s.threads == 64) f(E{}, std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
   else if (s.threads == 256) f(E{}, std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
+  else if (s.held == 4) f(E{}, std::integral_constant<int, 512>{}, std::integral_constant<int, 4>{});
   else f(E{}, std::integral_constant<int, 512>{}, std::integral_constant<int, 8>{});
 }
 template <typename F>
