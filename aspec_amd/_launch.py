@@ -35,7 +35,7 @@ class IndexFlags:
     stream, `raise_if_bad` waits for it and raises ValueError where an index was bad."""
 
     def __init__(self, device: torch.device):
-        self._home = _pool[device.index]
+        self.device, self._home = device, _pool[device.index]
         self._slot = None
         for _ in range(min(2, len(self._home))):  # the oldest first; one still pending goes to the end
             with contextlib.suppress(IndexError):
@@ -63,17 +63,25 @@ class IndexFlags:
             self._home.append(self._slot)
 
 
+def _capturing(device: torch.device) -> bool:
+    """Whether the device's current stream is being captured into a graph."""
+    if torch.cuda.current_device() == device.index:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def index_flags(wanted: bool, device: torch.device) -> IndexFlags | None:
     """The flags of a launch whose indices are to be checked. None where nothing can read them: the
     caller wants no check, or the launch is captured into a graph, whose replays no host follows."""
-    if not wanted or torch.cuda.is_current_stream_capturing():
+    if not wanted or _capturing(device):
         return None
     return IndexFlags(device)
 
 
 def settle(flags: IndexFlags | None) -> None:
     """Reads a deferred check behind the launches that it was deferred for."""
-    if flags is not None and not torch.cuda.is_current_stream_capturing():
+    if flags is not None and not _capturing(flags.device):
         flags.raise_if_bad()
 
 

@@ -572,8 +572,8 @@ int check_rows(int dtype, int64_t rows, int64_t vocab, int64_t row_stride, float
   if (vocab > kMaxVocab)
     return set_error(ASPEC_ERR_UNSUPPORTED, "token log-probabilities support at most %d logits per row",
                      static_cast<int>(kMaxVocab));
-  if (!(temperature > 0.f) || !(1.f / temperature > 0.f) || isinf(1.f / temperature))
-    return set_error(ASPEC_ERR_INVALID, "temperature must be finite and > 0");
+  if (!usable_temperature(temperature))
+    return set_error(ASPEC_ERR_INVALID, "temperature must be > 0, and its inverse a normal number");
   if (top_k < 0 || top_k > vocab)
     return set_error(ASPEC_ERR_INVALID, "top_k must lie in [0, vocab]");
   if (top_k > kMaxTop)

@@ -258,6 +258,7 @@ __device__ __forceinline__ void finish_row(const Args& a, int64_t row, int lane,
     kl += r * (log64(static_cast<float>(r)) - log_tail);
     accept += fminf(static_cast<float>(r), in_row / S);
   }
+  accept = fminf(accept, 1.f);  // but for the rounding of the log-probabilities it is
   if (empty) {
     kl = mass > 0. ? static_cast<double>(INFINITY) : 0.;
     accept = 0.f;

@@ -152,7 +152,7 @@ void launch_bwd(const Args& a, bool two, hipStream_t stream) {
 }
 
 int check_distill(int dtype, int64_t rows, int64_t vocab, int64_t row_stride, int token_dtype, int64_t kept,
-                  float temperature) {
+                  const int64_t* teacher_rows, int64_t num_teacher_rows, float temperature) {
   if (dtype != ASPEC_MASK_BF16 && dtype != ASPEC_MASK_F16 && dtype != ASPEC_MASK_F32)
     return set_error(ASPEC_ERR_UNSUPPORTED, "top-logit distillation takes bf16, fp16 or fp32 logits");
   if (rows < 0 || vocab <= 0 || row_stride < vocab)
@@ -162,11 +162,13 @@ int check_distill(int dtype, int64_t rows, int64_t vocab, int64_t row_stride, in
                      static_cast<int>(kMaxVocab));
   if (token_dtype != ASPEC_MASK_I64 && token_dtype != ASPEC_MASK_I32)
     return set_error(ASPEC_ERR_INVALID, "teacher tokens are int64 or int32");
+  if (teacher_rows ? num_teacher_rows < 1 && rows > 0 : num_teacher_rows != rows)
+    return set_error(ASPEC_ERR_INVALID, "a teacher has a row per logit row, or a table of at least one");
   if (kept < 1) return set_error(ASPEC_ERR_INVALID, "top-logit distillation needs a teacher token per row");
   if (kept > kMaxTop)
     return set_error(ASPEC_ERR_UNSUPPORTED, "at most %d teacher tokens per row are supported", kMaxTop);
-  if (!(temperature > 0.f) || !(1.f / temperature > 0.f) || isinf(1.f / temperature))
-    return set_error(ASPEC_ERR_INVALID, "temperature must be finite and > 0");
+  if (!usable_temperature(temperature))
+    return set_error(ASPEC_ERR_INVALID, "temperature must be > 0, and its inverse a normal number");
   return ASPEC_OK;
 }
 
@@ -226,7 +228,7 @@ using namespace aspec;
 extern "C" int aspec_topk_distill_stats_floats(void) { return kStats; }
 
 extern "C" int aspec_topk_distill_workspace_bytes(int dtype, int64_t rows, int64_t vocab, size_t* bytes) {
-  if (const int e = check_distill(dtype, rows, vocab, vocab, ASPEC_MASK_I64, 1, 1.f)) return e;
+  if (const int e = check_distill(dtype, rows, vocab, vocab, ASPEC_MASK_I64, 1, nullptr, rows, 1.f)) return e;
   if (!bytes) return null_pointer();
   const Shape s = shape_of(rows, vocab, per_chunk_of(dtype));
   *bytes = s.parts == 1 ? 0 : static_cast<size_t>(rows) * s.parts * (4 * 4 + 8);
@@ -243,7 +245,9 @@ extern "C" int aspec_topk_distill_fwd(const void* logits, int dtype, int64_t row
                                       const int64_t* teacher_rows, int64_t num_teacher_rows, int renormalize,
                                       float temperature, float* ce, float* kl, float* accept, int64_t* argmax,
                                       float* stats, void* workspace, int32_t* status_words, void* stream) {
-  if (const int e = check_distill(dtype, rows, vocab, row_stride, token_dtype, kept, temperature)) return e;
+  if (const int e = check_distill(dtype, rows, vocab, row_stride, token_dtype, kept, teacher_rows, num_teacher_rows,
+                                  temperature))
+    return e;
   if (rows == 0) return ASPEC_OK;
   const Args a = make_args(logits, dtype, rows, vocab, row_stride, targets, ignore_index, teacher_tokens, token_dtype,
                            teacher_logprobs, kept, teacher_rows, num_teacher_rows, renormalize, temperature, ce, kl,
@@ -261,7 +265,9 @@ extern "C" int aspec_topk_distill_bwd(const void* logits, int dtype, int64_t row
                                       const int64_t* teacher_rows, int64_t num_teacher_rows, float temperature,
                                       const float* stats, const float* grad_ce, const float* grad_kl,
                                       void* grad_logits, int64_t grad_stride, void* stream) {
-  if (const int e = check_distill(dtype, rows, vocab, row_stride, token_dtype, kept, temperature)) return e;
+  if (const int e = check_distill(dtype, rows, vocab, row_stride, token_dtype, kept, teacher_rows, num_teacher_rows,
+                                  temperature))
+    return e;
   if (grad_stride < vocab)
     return set_error(ASPEC_ERR_INVALID, "top-logit distillation needs a vocabulary and rows at least as far apart");
   if (rows == 0) return ASPEC_OK;
@@ -286,7 +292,9 @@ extern "C" int aspec_topk_distill_fused_fwd_bwd(
     const int64_t* teacher_rows, int64_t num_teacher_rows, int renormalize, float temperature, const float* grad_ce,
     const float* grad_kl, float* ce, float* kl, float* accept, int64_t* argmax, float* stats, void* workspace,
     void* grad_logits, int64_t grad_stride, int32_t* status_words, void* stream) {
-  if (const int e = check_distill(dtype, rows, vocab, row_stride, token_dtype, kept, temperature)) return e;
+  if (const int e = check_distill(dtype, rows, vocab, row_stride, token_dtype, kept, teacher_rows, num_teacher_rows,
+                                  temperature))
+    return e;
   if (grad_stride < vocab)
     return set_error(ASPEC_ERR_INVALID, "top-logit distillation needs a vocabulary and rows at least as far apart");
   if (rows == 0) return ASPEC_OK;

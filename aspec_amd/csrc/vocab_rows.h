@@ -343,6 +343,9 @@ struct Shape {
 };
 constexpr int64_t kMaxVocab = int64_t{1} << 19;  // 32 parts of 4096 chunks of four fp32 logits
 
+// Whether 1 / temperature is a normal number (a subnormal one is 0 to the kernels).
+inline bool usable_temperature(float t) { return t > 0.f && 1.f / t >= 0x1p-126f && !isinf(1.f / t); }
+
 inline int per_chunk_of(int dtype) { return dtype == ASPEC_MASK_F32 ? 4 : 8; }
 
 // Rows of up to 256 chunks take a wave each, up to 1024 a workgroup of 256 threads. Longer rows take

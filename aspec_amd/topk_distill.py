@@ -211,4 +211,6 @@ def _fused(logits, targets, teacher_indices, teacher_logprobs, ce_weights, kl_we
            call.renormalize, call.temperature, ptr(weights[0]), ptr(weights[1]), ptr(ce), kl.data_ptr(),
            accept.data_ptr(), ptr(amax), ptr(stats), ptr(workspace), grad.data_ptr(), row_stride(grad),
            None if flags is None else flags.ptr)
+    if in_place and not logits.is_inference():
+        torch.autograd.graph.increment_version(logits)  # a graph that kept the logits must not use them
     return (ce, kl, accept, logits if in_place else grad.view(logits.shape), amax), flags

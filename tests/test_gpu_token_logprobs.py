@@ -332,3 +332,34 @@ def test_saved_tensors_that_move(gpu):
     twice.mul_(2)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         out.logprobs.sum().backward()
+
+
+def test_more_rows_than_a_grid_is_wide(gpu):
+    """2^21 workgroups are one line of the grid: rows past them, small vocabularies."""
+    rows, vocab = 2 ** 21 + 5, 8
+    x, g = logits(gpu, rows, vocab, torch.bfloat16, 99)
+    ids = torch.randint(0, vocab, (rows,), device=gpu, generator=g)
+    leaf = x.requires_grad_()
+    out = token_logprobs(leaf, ids, top_k=3)
+    (dx,) = torch.autograd.grad(out.logprobs.sum(), leaf)
+    want = torch.log_softmax(x.detach().double(), -1)
+    torch.testing.assert_close(out.logprobs.double(), want.gather(1, ids[:, None])[:, 0], atol=STEPS, rtol=4 * U)
+    assert torch.equal(out.top_indices, x.detach().float().sort(dim=-1, descending=True, stable=True).indices[:, :3])
+    ref = torch.nn.functional.one_hot(ids, vocab) - want.exp()
+    torch.testing.assert_close(dx.double(), ref, atol=4 * STEPS, rtol=2.0 ** -8)
+
+
+@pytest.mark.parametrize("temperature", [1e-3, 1e-30, 1e30])
+def test_extreme_temperatures(gpu, temperature):
+    """Nearly all or nearly none of the spread: the largest tokens share everything, or all tokens do."""
+    x, g = logits(gpu, 3, 700, torch.float32, 100)
+    x[1, 5] = -float("inf")
+    x[2, [7, 9]] = 30.0
+    out = token_logprobs(x, torch.tensor([0, 5, 9], device=gpu), top_k=4, temperature=temperature)
+    if temperature < 1:
+        assert out.logprobs[2].item() == pytest.approx(-np.log(2), abs=STEPS)
+        assert out.entropy.tolist() == pytest.approx([0.0, 0.0, np.log(2)], abs=2 * STEPS)
+    else:
+        assert out.logprobs[0].item() == pytest.approx(-np.log(700), abs=2 * STEPS)
+        assert out.entropy.tolist() == pytest.approx([np.log(700), np.log(699), np.log(700)], abs=16 * STEPS)
+    assert out.logprobs[1].item() == -float("inf")

@@ -411,3 +411,48 @@ def test_saved_tensors_that_move(gpu):
     case.logprobs.sub_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         kl.sum().backward()
+
+
+def test_more_rows_than_a_grid_is_wide(gpu):
+    """2^21 workgroups are one line of the grid: rows past them equal the same rows alone."""
+    rows, vocab = 2 ** 21 + 6, 9
+    tail = Case(gpu, 6, vocab, 4, torch.float32, 99)
+    x = torch.zeros(rows, vocab, device=gpu)
+    x[-6:] = tail.x
+    index = torch.zeros(rows, dtype=torch.int64, device=gpu)
+    index[-6:] = torch.arange(6, device=gpu)
+    targets = torch.zeros(rows, dtype=torch.int64, device=gpu)
+    targets[-6:] = tail.targets
+    weights = torch.zeros(2, rows, device=gpu)
+    weights[0, -6:], weights[1, -6:] = tail.g_ce, tail.g_kl
+    leaf = x.requires_grad_()
+    ce, kl, accept = topk_distill_from_logits(leaf, targets, tail.tokens, tail.logprobs, teacher_rows=index)
+    (dx,) = torch.autograd.grad([ce, kl], leaf, [weights[0], weights[1]])
+    fused = topk_distill_fused_grad(x.detach(), targets, tail.tokens, tail.logprobs, ce_weights=weights[0],
+                                    kl_weights=weights[1], teacher_rows=index)
+    (r_ce, r_kl, r_accept, _), (grad, size) = tail.oracle()
+    for got in ((ce, kl, accept, dx), fused):
+        _close(got[0][-6:], r_ce, STEPS + 4 * U * np.abs(r_ce), "ce")
+        _close(got[1][-6:], r_kl, 3 * STEPS * (1 + np.abs(r_kl)), "kl")
+        _close(got[2][-6:], r_accept, 2 * STEPS, "accept")
+        _close(got[3][-6:], grad, HALF[torch.float32] * np.abs(grad) + 3 * STEPS * size + 1e-37, "grad")
+        assert (got[3][:-6] == 0).all()
+
+
+def test_in_place_is_seen_by_autograd(gpu):
+    """A graph that kept the logits does not use the gradient that has taken their place."""
+    case = Case(gpu, 4, 500, 5, torch.float32, 101)
+    leaf = case.x.clone().requires_grad_()
+    logits = leaf * 1.0
+    square = (logits * logits).sum()
+    topk_distill_fused_grad(logits, case.targets, case.tokens, case.logprobs, ce_weights=case.g_ce,
+                            kl_weights=case.g_kl, in_place=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        square.backward()
+    with torch.inference_mode():  # no graph, no versions
+        x = case.x.clone()
+        out = topk_distill_fused_grad(x, case.targets, case.tokens, case.logprobs, ce_weights=case.g_ce,
+                                      kl_weights=case.g_kl, in_place=True)
+        assert out[3].data_ptr() == x.data_ptr() and torch.equal(x, logits.detach())
+        assert torch.equal(topk_distill_from_logits(case.x, case.targets, case.tokens, case.logprobs)[1], out[1])
+        assert token_logprobs(case.x, top_k=3).top_indices.shape == (4, 3)

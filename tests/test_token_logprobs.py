@@ -89,7 +89,7 @@ def test_refusals_of_the_c_entries():
             fwd(**bad)
     with pytest.raises(NotImplementedError, match="524288"):
         fwd(vocab=524289, stride=524289)
-    for temperature in (0.0, -1.0, float("nan"), float("inf"), 1e-45):
+    for temperature in (0.0, -1.0, float("nan"), float("inf"), 1e-45, 3e38):
         with pytest.raises(ValueError, match="temperature"):
             fwd(temperature=temperature)
     for top_k in (-1, 101):

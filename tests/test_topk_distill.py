@@ -110,8 +110,10 @@ def test_refusals_of_the_c_entries():
     fake, other = ctypes.c_void_p(4096), ctypes.c_void_p(8192)  # never dereferenced: every call fails its checks
 
     def calls(dtype=4, rows=2, vocab=100, stride=100, token_dtype=1, kept=5, temperature=1.0, logits=fake, targets=fake,
-              tokens=fake, ce=fake, stats=fake, grad=other, grad_stride=100, workspace=None, which="fwd bwd fused"):
-        head = (logits, dtype, rows, vocab, stride, targets, -100, tokens, token_dtype, fake, kept, None, rows)
+              tokens=fake, ce=fake, stats=fake, grad=other, grad_stride=100, workspace=None, teacher_rows=None,
+              num_teacher_rows=None, which="fwd bwd fused"):
+        head = (logits, dtype, rows, vocab, stride, targets, -100, tokens, token_dtype, fake, kept, teacher_rows,
+                rows if num_teacher_rows is None else num_teacher_rows)
         if "fwd" in which:
             yield lib.aspec_topk_distill_fwd(*head, 0, temperature, ce, fake, fake, None, stats, workspace, None, None)
         if "bwd" in which:
@@ -133,7 +135,9 @@ def test_refusals_of_the_c_entries():
     refused(ValueError, "int64 or int32", token_dtype=4)
     refused(ValueError, "a teacher token per row", kept=0)
     refused(NotImplementedError, "128", kept=129)
-    for temperature in (0.0, -1.0, float("nan"), float("inf"), 1e-45):
+    refused(ValueError, "a table of at least one", teacher_rows=fake, num_teacher_rows=0)
+    refused(ValueError, "a table of at least one", num_teacher_rows=3)
+    for temperature in (0.0, -1.0, float("nan"), float("inf"), 1e-45, 3e38):
         refused(ValueError, "temperature", temperature=temperature)
     for bad in ({"logits": None}, {"tokens": None}):
         refused(ValueError, "null pointer", **bad)
