@@ -173,7 +173,7 @@ __global__ __launch_bounds__(T, 8) void token_logprobs_kernel(FwdArgs a) {
   using P = Part<E, T, NV>;
   constexpr int W = T / 64;
   __shared__ float s_m[W], s_S[W], s_D[W];
-  __shared__ uint16_t s_reach[TOP ? T : 1];  // threads whose maximum reaches the bound
+  __shared__ uint16_t s_reach[TOP ? T * NV : 1];  // chunks whose maximum reaches the bound
   __shared__ uint32_t s_reached;
   __shared__ uint32_t s_best[TOP ? T : 1], s_count[W];
   __shared__ uint32_t s_n, s_bound, s_high;
@@ -285,8 +285,8 @@ __global__ __launch_bounds__(T, 8) void token_logprobs_kernel(FwdArgs a) {
       }
     }
     __syncthreads();
-    // ---- the list: the chunks of the few threads whose maximum reaches the bound are dealt out to all
-    // threads, which read them again (from L2) and list what reaches it
+    // ---- the list: the few chunks whose largest token reaches the bound are dealt out to all threads,
+    // which read them again and list what reaches it
     const uint32_t bound = s_bound;
     const float bound_value = key_value(bound);  // a NaN bound lists every token
     const int chunks = P::chunks_in(cut, part, a.part_chunks);
@@ -294,13 +294,17 @@ __global__ __launch_bounds__(T, 8) void token_logprobs_kernel(FwdArgs a) {
       const uint32_t slot = atomicAdd(&s_n, 1u);
       if (slot < kList) s_list[slot] = ranked(order_key(v), at);
     };
-    if (!(m < bound_value) || S != S) s_reach[atomicAdd(&s_reached, 1u)] = static_cast<uint16_t>(threadIdx.x);
+    if (!(m < bound_value) || S != S) {
+      uint32_t reach = S != S ? (1u << NV) - 1 : p.chunks_reaching(bound_value);  // the maxima skip a NaN
+      for (; reach; reach &= reach - 1)
+        s_reach[atomicAdd(&s_reached, 1u)] = static_cast<uint16_t>(threadIdx.x + __builtin_ctz(reach) * T);
+    }
     if (p.edge_at >= 0 && !(p.edge < bound_value)) append(p.edge, p.edge_at);
     __syncthreads();
-    const int tasks = static_cast<int>(s_reached) * NV;
+    const int tasks = s_reached;
     for (int task = threadIdx.x; task < tasks; task += T) {
       if (*static_cast<volatile uint32_t*>(&s_n) > kList) break;  // the list is lost already
-      const int c = s_reach[task / NV] + (task % NV) * T;
+      const int c = s_reach[task];
       if (c >= chunks) continue;
       const int first = P::index_of(cut, part, a.part_chunks, c);
       const uint4 w = load16<E>(x, first);

@@ -177,23 +177,24 @@ struct Part {
     asm volatile("" : "+v"(held), "+v"(first));
   }
 
-  // The thread's largest element; a NaN is skipped, or is the result. Sixteen-bit floats are compared
-  // as whole numbers, two to an instruction and without widening: where any is positive, the largest
-  // number is the largest float; where none is, the smallest number is.
-  __device__ __forceinline__ float largest() const {
+  // The largest element of chunks [from, to) of the thread; a NaN is skipped, or is the result.
+  // Sixteen-bit floats are compared as whole numbers, two to an instruction and without widening:
+  // where any is positive, the largest number is the largest float; where none is, the smallest is.
+  template <int FROM, int TO>
+  __device__ __forceinline__ float largest_of() const {
     if constexpr (CH == 4) {
-      float m = edge;
+      float m = kNegInf;
 #pragma unroll
-      for (int v = 0; v < NV; ++v)
+      for (int v = FROM; v < TO; ++v)
 #pragma unroll
         for (int i = 0; i < CH; ++i) m = fmaxf(m, element<E>(w[v], i));
       return m;
     } else {
       typedef __attribute__((ext_vector_type(2))) short pair;
       const auto fold = [&](auto op) {
-        pair r = __builtin_bit_cast(pair, w[0].x);
+        pair r = __builtin_bit_cast(pair, w[FROM].x);
 #pragma unroll
-        for (int v = 0; v < NV; ++v)
+        for (int v = FROM; v < TO; ++v)
 #pragma unroll
           for (int j = 0; j < 4; ++j) r = op(r, __builtin_bit_cast(pair, word_of(w[v], j)));
         return r;
@@ -204,7 +205,17 @@ struct Part {
         const pair low = fold([](pair a, pair b) { return __builtin_elementwise_min(a, b); });
         best = low.x < low.y ? low.x : low.y;
       }
-      return fmaxf(E::widen(static_cast<uint16_t>(best)), edge);
+      return E::widen(static_cast<uint16_t>(best));
+    }
+  }
+  __device__ __forceinline__ float largest() const { return fmaxf(largest_of<0, NV>(), edge); }
+  // One bit for each chunk whose largest element is not below a bound.
+  template <int V = 0>
+  __device__ __forceinline__ uint32_t chunks_reaching(float bound) const {
+    if constexpr (V < NV) {
+      return (largest_of<V, V + 1>() < bound ? 0u : 1u << V) | chunks_reaching<V + 1>(bound);
+    } else {
+      return 0;
     }
   }
 
