@@ -8,8 +8,10 @@
 //
 // HBM-bound: the forward reads each logit once, the backward reads it once and writes the gradient
 // once. A row (or a part of a long one) lies in registers while its maximum, sums and best tokens
-// are taken. 8192 x 32000 bf16: forward 92 us (5.7 TB/s; leaving out the exponentials or the entropy
-// does not shorten it), backward 171 us (6.1 TB/s read and written).
+// are taken. 8192 x 32000 bf16: forward 92 us back to back (5.7 TB/s; leaving out the exponentials or
+// the entropy does not shorten it) and 111-130 behind 524 MB of gradient writes, backward 171 us
+// (6.1 TB/s read and written). Holding the next row's loads in flight as well was slower (113 us against
+// 128: 95 registers leave two workgroups to a CU in place of four).
 //
 // The K best: at least K tokens are >= the K-th largest of the maxima of groups of threads, and few
 // more than K of them are unless the large ones share groups. One wave finds that bound by bisection
@@ -18,11 +20,13 @@
 // ~index) as one 64-bit number, no two alike. A list that overflows (long runs of equal logits,
 // large ones that share threads) is replaced by exactly the K best: the K-th largest value, found by
 // bisection with counts over the part, and its ties in order.
-// 4096 x 32000 bf16 with the 64 best: 63 us against 46 without them. What is left is the chain behind
-// a row's last load (four barriers, the bisection, the list, the places; about 4 us), in which its
-// workgroup asks for nothing, with four workgroups to a CU; asking for the next row ahead of it costs
-// the registers of two of the four, and was slower (95 us). 8192 x 32000, 64 best: random 131 us, all
-// equal 390, all but 40 masked 436, ascending (the list overflows, and 64-fold ties) 1080.
+// 4096 x 32000 bf16 with the 64 best: 61 us against 46 without them, 288 MB read (the row, and the
+// chunks of the listed tokens again). What is left is the chain behind a row's last load (four
+// barriers, the bisection, the list, the places; about 4 us), in which its workgroup asks for nothing,
+// with four workgroups to a CU; asking for the next row ahead of it costs the registers of two of the
+// four, and was slower (95 us). 8192 x 32000: random 87 us without alternatives, 102 with 1, 110 with
+// 20, 117 with 64, 155 with 128; 64 of rows that are all equal 400, of rows masked but for 40 tokens
+// 434, of ascending rows (the list overflows, and 64-fold ties) 1066.
 #include "vocab_rows.h"
 
 namespace aspec {
@@ -30,7 +34,7 @@ namespace {
 
 using namespace vocab;
 
-constexpr int kStats = 4;       // per row: maximum, S, entropy, D / S
+constexpr int kStats = 4;       // per row: maximum, S, D / S, 0 (16 bytes)
 constexpr int kList = 512;      // tokens at or above the bound that are ranked without a search
 
 struct FwdArgs {
@@ -104,7 +108,7 @@ __device__ __forceinline__ RowResult finish_row(const FwdArgs& a, int64_t row, c
     const float entropy = empty ? 0.f : log_s - kLn2 * s.D / s.S;
     a.entropy[row] = entropy;
     if (a.stats)
-      *reinterpret_cast<float4*>(a.stats + row * kStats) = make_float4(s.m, s.S, entropy, empty ? 0.f : s.D / s.S);
+      *reinterpret_cast<float4*>(a.stats + row * kStats) = make_float4(s.m, s.S, empty ? 0.f : s.D / s.S, 0.f);
     if (a.ids) {
       float lp = 0.f;
       if (id != a.ignore_index) {
@@ -547,7 +551,7 @@ __global__ __launch_bounds__(T, 8) void token_logprobs_bwd_kernel(BwdArgs a) {
   }
   // logp + H = ln2 (d - D / S), so dx = e (u + v d) with e = exp2(d)
   const float v = -gh * kLn2 * inv_s * a.inv_t;
-  const float u = empty ? 0.f : (gh * kLn2 * st.w - lost) * inv_s * a.inv_t;
+  const float u = empty ? 0.f : (gh * kLn2 * st.z - lost) * inv_s * a.inv_t;
   const auto dense = [&](float xv) {
     const float d = (xv - base) * scale, e = fast_exp2(d);
     if constexpr (ENTROPY) return e * fmaf(v, fmaxf(d, -200.f), u);

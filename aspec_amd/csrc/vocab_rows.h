@@ -379,8 +379,9 @@ inline Shape shape_of(int64_t rows, int64_t V, int per_chunk) {
   return s;
 }
 
-// Waves per SIMD that the compiler keeps registers for: three workgroups of 512 threads to a CU (80
-// registers), so that one's reductions and searches hide behind another's loads; one of 1024 (128).
+// Waves per SIMD that the compiler keeps registers for where a workgroup holds a row for its losses and
+// its gradient: three workgroups of 512 threads to a CU (80 registers), so that one's reductions hide
+// behind another's loads; one of 1024 (128). Kernels without the gradient fit eight waves (64).
 constexpr int min_waves(int threads) { return threads == 1024 ? 4 : 6; }
 
 // One workgroup per unit (a row or a part of one), not a loop over units: what a loop body of this
