@@ -79,6 +79,18 @@ def index_flags(wanted: bool, device: torch.device) -> IndexFlags | None:
     return IndexFlags(device)
 
 
+# From this many bytes of logits a call that has to read its check before it returns has its indices
+# checked by a kernel of their own, ahead of the logits' pass, and waits for that one: the pass then runs
+# on while the host prepares the next call. bf16 rows of 32000, us a call (a call that the GPU is waited
+# for behind): 2048 of them, losses and gradient, 64 (100) so and 92 (96) with the check in the pass;
+# 256 of them 46 (63) and 53 (59).
+CHECK_FIRST_BYTES = 1 << 25
+
+
+def check_first(flags: IndexFlags | None, logits: torch.Tensor) -> bool:
+    return flags is not None and logits.numel() * logits.element_size() >= CHECK_FIRST_BYTES
+
+
 def settle(flags: IndexFlags | None) -> None:
     """Reads a deferred check behind the launches that it was deferred for."""
     if flags is not None and not _capturing(flags.device):

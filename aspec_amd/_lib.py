@@ -84,6 +84,7 @@ SIGNATURES = {
     "aspec_sampled_l1_bwd": (_int, [_c_void_p] * 3 + [_i64, _i64, _i64] + [_c_void_p] * 4),
     "aspec_token_logprobs_stats_floats": (_int, []),
     "aspec_token_logprobs_workspace_bytes": (_int, [_int, _i64, _i64, _i64, _size_p]),
+    "aspec_token_logprobs_check": (_int, [_c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p]),
     "aspec_token_logprobs_fwd": (
         _int, [_c_void_p, _int, _i64, _i64, _i64, _c_void_p, _i64, _f32, _i64] + [_c_void_p] * 8
     ),
@@ -94,6 +95,9 @@ SIGNATURES = {
     "aspec_topk_distill_stats_floats": (_int, []),
     "aspec_topk_distill_workspace_bytes": (_int, [_int, _i64, _i64, _size_p]),
     "aspec_topk_distill_reads": (_int, [_int, _i64]),
+    "aspec_topk_distill_check": (
+        _int, [_i64, _i64, _c_void_p, _i64, _c_void_p, _int, _c_void_p, _i64, _c_void_p, _i64, _c_void_p, _c_void_p]
+    ),
     "aspec_topk_distill_fwd": (
         _int, [_c_void_p, _int, _i64, _i64, _i64, _c_void_p, _i64, _c_void_p, _int, _c_void_p, _i64, _c_void_p,
                _i64, _int, _f32] + [_c_void_p] * 8

@@ -574,6 +574,16 @@ __global__ __launch_bounds__(T, 8) void token_logprobs_bwd_kernel(BwdArgs a) {
     dx[given] = E::narrow(dense(E::widen(raw_given)) + g_given * direct);
 }
 
+// The tokens' range alone: a host that must know before it goes on waits for this and not for the
+// logits' pass queued behind it.
+__global__ __launch_bounds__(256) void token_logprobs_check_kernel(const int64_t* ids, int64_t rows, int64_t V,
+                                                                   int64_t ignore_index, int32_t* status) {
+  const int64_t row = unit_of_block() * 256 + threadIdx.x;
+  if (row >= rows) return;
+  const int64_t id = ids[row];
+  if (id != ignore_index && (id < 0 || id >= V)) report(status, kBadTokenId);
+}
+
 template <typename E, int T, int NV>
 void launch_fwd(const FwdArgs& a, hipStream_t stream) {
   const dim3 grid = grid_of(a.rows * a.parts);
@@ -624,6 +634,17 @@ extern "C" int aspec_token_logprobs_workspace_bytes(int dtype, int64_t rows, int
   const vocab::Shape s = vocab::shape_of(rows, vocab, vocab::per_chunk_of(dtype));
   *bytes = s.parts == 1 ? 0 : static_cast<size_t>(rows) * s.parts * (top_k * 8 + 3 * 4);
   return ASPEC_OK;
+}
+
+extern "C" int aspec_token_logprobs_check(const int64_t* token_ids, int64_t rows, int64_t vocab, int64_t ignore_index,
+                                          int32_t* status_words, void* stream) {
+  if (const int e = check_rows(ASPEC_MASK_F32, rows, vocab, vocab, 1.f, 0)) return e;
+  if (rows == 0) return ASPEC_OK;
+  if (!token_ids || !status_words)
+    return set_error(ASPEC_ERR_INVALID, "null pointer passed to token log-probabilities");
+  token_logprobs_check_kernel<<<vocab::grid_of((rows + 255) / 256), 256, 0, static_cast<hipStream_t>(stream)>>>(
+      token_ids, rows, vocab, ignore_index, status_words);
+  return check_launch("token_logprobs_check_kernel");
 }
 
 extern "C" int aspec_token_logprobs_fwd(const void* logits, int dtype, int64_t rows, int64_t vocab,

@@ -139,6 +139,48 @@ __global__ __launch_bounds__(T, 8) void topk_distill_bwd_kernel(Args a) {
         E::narrow(st[1] == 0.f ? 0.f : f.template tail<TWO>(E::widen(raw_target), scale) - gc);
 }
 
+// The indices alone, a wave to a row: what is wrong with them goes to the status words. It reads a few
+// hundred bytes a row (8192 rows of 64 tokens: 4 us), so a host that must know before it goes on waits
+// for this and not for the logits' pass queued behind it.
+constexpr int kCheckRows = 4;
+constexpr int kSeenBits = 1 << 15;
+__global__ __launch_bounds__(64 * kCheckRows) void topk_distill_check_kernel(Args a) {
+  __shared__ uint4 s_seen[kCheckRows][kSeenBits / 128];
+  const int lane = threadIdx.x & 63;
+  const int64_t row = unit_of_block() * kCheckRows + (threadIdx.x >> 6);
+  const bool live = row < a.rows;
+  const int64_t trow = live ? teacher_row(a, row) : -1;  // no row: no token
+  const bool bad_target = live && read_target(a, row).bad;
+  bool bad = false;
+  int token[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) token[h] = token_of(a, trow, lane + 64 * h, load_entry(a, trow, lane + 64 * h), bad);
+  // a token that finds its bit (its index modulo 2^15) set may be there twice, and is counted
+  uint4* words = s_seen[threadIdx.x >> 6];
+#pragma unroll
+  for (int i = 0; i < kSeenBits / 128 / 64; ++i) words[lane + 64 * i] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+  bool twice = false;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    bool seen = false;
+    if (token[h] >= 0) {
+      const uint32_t bit = 1u << (token[h] & 31);
+      seen = (atomicOr(reinterpret_cast<uint32_t*>(words) + (token[h] % kSeenBits >> 5), bit) & bit) != 0;
+    }
+    for (uint64_t lanes = __ballot(seen); lanes; lanes &= lanes - 1) {
+      const int t = __builtin_amdgcn_readlane(token[h], __ffsll(static_cast<unsigned long long>(lanes)) - 1);
+      twice |= __popcll(__ballot(token[0] == t)) + __popcll(__ballot(token[1] == t)) > 1;
+    }
+  }
+  const bool any_bad = __any(bad);
+  if (lane != 0 || !live) return;
+  if (trow < 0) report(a.status, kBadTeacherRow);
+  if (bad_target) report(a.status, kBadTarget);
+  if (any_bad) report(a.status, kBadTeacherToken);
+  if (twice) report(a.status, kRepeatedToken);
+}
+
 template <typename E, int T, int NV>
 void launch_fwd(const Args& a, bool two, hipStream_t stream) {
   const dim3 grid = grid_of(a.rows * a.parts);
@@ -242,6 +284,23 @@ extern "C" int aspec_topk_distill_workspace_bytes(int dtype, int64_t rows, int64
 
 extern "C" int aspec_topk_distill_reads(int dtype, int64_t vocab) {
   return topk_distill_fused_fits(vocab, per_chunk_of(dtype)) ? 1 : 2;
+}
+
+extern "C" int aspec_topk_distill_check(int64_t rows, int64_t vocab, const int64_t* targets, int64_t ignore_index,
+                                        const void* teacher_tokens, int token_dtype, const float* teacher_logprobs,
+                                        int64_t kept, const int64_t* teacher_rows, int64_t num_teacher_rows,
+                                        int32_t* status_words, void* stream) {
+  if (const int e = check_distill(ASPEC_MASK_F32, rows, vocab, vocab, token_dtype, kept, teacher_rows,
+                                  num_teacher_rows, 1.f))
+    return e;
+  if (rows == 0) return ASPEC_OK;
+  if (!teacher_tokens || !teacher_logprobs || !status_words) return null_pointer();
+  const Args a = make_args(nullptr, ASPEC_MASK_F32, rows, vocab, vocab, targets, ignore_index, teacher_tokens,
+                           token_dtype, teacher_logprobs, kept, teacher_rows, num_teacher_rows, 0, 1.f, nullptr,
+                           nullptr, nullptr, nullptr, nullptr, nullptr, status_words);
+  topk_distill_check_kernel<<<grid_of((rows + kCheckRows - 1) / kCheckRows), 64 * kCheckRows, 0,
+                              static_cast<hipStream_t>(stream)>>>(a);
+  return check_launch("topk_distill_check_kernel");
 }
 
 extern "C" int aspec_topk_distill_fwd(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,

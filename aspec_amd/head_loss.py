@@ -116,7 +116,7 @@ class _SelectiveHeadDistillation(torch.autograd.Function):
             torch.cuda.current_stream(hidden.device).wait_event(teacher_ready)
         (ce, kl, accept, dlogits, amax), ctx.flags = _topk_distill_fused(
             logits, targets, indices, logprobs, ce_weights, kl_weights, teacher_rows, tail, temperature, ignore_index,
-            want_argmax, True, True)
+            want_argmax, True, True, not has_backward)
         if not has_backward:
             settle(ctx.flags)
         objective = torch.dot(kl_weights.float(), kl)

@@ -26,7 +26,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from aspec_amd import _lib
-from aspec_amd._launch import index_flags, launch, settle
+from aspec_amd._launch import check_first, index_flags, launch, settle
 
 # ASPEC_MASK_* codes of the logits' types
 LOGIT_CODES = {torch.float32: 0, torch.bfloat16: 4, torch.float16: 5}
@@ -109,10 +109,14 @@ def _forward(logits, ids, top_k, temperature, ignore_index, check_ids, has_backw
     top_indices = torch.empty((*lead, top_k), dtype=torch.int64, device=dev) if top_k else None
     stats = torch.empty((rows, stat_floats), dtype=torch.float32, device=dev) if has_backward else None
     flags = index_flags(check_ids and ids is not None, dev)
-    ptr = _lib.ptr
-    launch("token_logprobs_fwd", dev, flags, "aspec_token_logprobs_fwd",
+    pass_flags, ptr = flags, _lib.ptr
+    if not has_backward and check_first(flags, flat):
+        launch("token_logprobs_check", dev, flags, "aspec_token_logprobs_check", ids.data_ptr(), rows, vocab,
+               ignore_index, flags.ptr)
+        pass_flags = None
+    launch("token_logprobs_fwd", dev, pass_flags, "aspec_token_logprobs_fwd",
            *_head(flat, ids, ignore_index, temperature, top_k), ptr(logprobs), entropy.data_ptr(), ptr(top),
-           ptr(top_indices), ptr(stats), ptr(workspace), None if flags is None else flags.ptr)
+           ptr(top_indices), ptr(stats), ptr(workspace), None if pass_flags is None else pass_flags.ptr)
     return (logprobs, entropy, top, top_indices), flat, stats, flags
 
 

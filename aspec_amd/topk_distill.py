@@ -27,7 +27,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from aspec_amd import _lib
-from aspec_amd._launch import index_flags, launch, settle
+from aspec_amd._launch import check_first, index_flags, launch, settle
 from aspec_amd.token_logprobs import LOGIT_CODES, check_temperature, float_grad, logit_rows, row_stride, vector
 
 _TAILS = {"bucket": 0, "renormalize": 1}
@@ -78,6 +78,17 @@ class _Call:
     def head(self, flat):
         return _head(flat, self.targets, self.ignore_index, self.indices, self.logprobs, self.teacher_rows)
 
+    def check(self, flat, flags, waits):
+        """The flags that are left to the logits' pass. Where the call `waits` for its check, the indices of
+        a long pass are checked ahead of it."""
+        if not waits or not check_first(flags, flat):
+            return flags
+        launch("topk_distill_check", flat.device, flags, "aspec_topk_distill_check", *flat.shape,
+               _lib.ptr(self.targets), self.ignore_index, self.indices.data_ptr(), _TOKEN_CODES[self.indices.dtype],
+               self.logprobs.data_ptr(), self.indices.shape[1], _lib.ptr(self.teacher_rows), self.indices.shape[0],
+               flags.ptr)
+        return None
+
     def outputs(self, flat, want_argmax, want_stats):
         """(ce, kl, accept_rate, argmax, stats, workspace) to be written; None where not wanted."""
         dev, lead = flat.device, self.lead
@@ -114,10 +125,10 @@ def _forward(logits, call, want_argmax, check, has_backward):
     flat = logit_rows(logits, "top-logit distillation")
     ce, kl, accept, amax, stats, workspace = call.outputs(flat, want_argmax, has_backward)
     flags = index_flags(check, flat.device)
-    ptr = _lib.ptr
-    launch("topk_distill_fwd", flat.device, flags, "aspec_topk_distill_fwd", *call.head(flat), call.renormalize,
+    pass_flags, ptr = call.check(flat, flags, not has_backward), _lib.ptr
+    launch("topk_distill_fwd", flat.device, pass_flags, "aspec_topk_distill_fwd", *call.head(flat), call.renormalize,
            call.temperature, ptr(ce), kl.data_ptr(), accept.data_ptr(), ptr(amax), ptr(stats), ptr(workspace),
-           None if flags is None else flags.ptr)
+           None if pass_flags is None else pass_flags.ptr)
     return (ce, kl, accept, amax), flat, stats, flags
 
 
@@ -183,14 +194,15 @@ def topk_distill_fused_grad(logits, targets, teacher_indices, teacher_logprobs, 
     with `targets`. With `in_place` the dlogits overwrite `logits`, which then are rows of adjacent
     elements. Rows too long for one workgroup (V > 163840, fp32: 81920) are read twice."""
     out, flags = _fused(logits, targets, teacher_indices, teacher_logprobs, ce_weights, kl_weights, teacher_rows, tail,
-                        temperature, ignore_index, return_argmax, in_place, check_indices)
+                        temperature, ignore_index, return_argmax, in_place, check_indices, True)
     settle(flags)
     return out if return_argmax else out[:4]
 
 
 def _fused(logits, targets, teacher_indices, teacher_logprobs, ce_weights, kl_weights, teacher_rows, tail, temperature,
-           ignore_index, return_argmax, in_place, check_indices):
-    """The launch behind `topk_distill_fused_grad`, its index flags still to be settled."""
+           ignore_index, return_argmax, in_place, check_indices, waits):
+    """The launch behind `topk_distill_fused_grad`, its index flags still to be settled: at once (`waits`),
+    or behind work that the caller queues first."""
     call = _Call(logits, targets, teacher_indices, teacher_logprobs, teacher_rows, tail, temperature, ignore_index)
     if (targets is None) != (ce_weights is None):
         raise ValueError("ce_weights go with targets")
@@ -206,11 +218,11 @@ def _fused(logits, targets, teacher_indices, teacher_logprobs, ce_weights, kl_we
     ce, kl, accept, amax, stats, workspace = call.outputs(flat, return_argmax, _read_twice(flat))
     grad = flat if in_place else torch.empty(flat.shape, dtype=flat.dtype, device=flat.device)
     flags = index_flags(check_indices, flat.device)
-    ptr = _lib.ptr
-    launch("topk_distill_fused", flat.device, flags, "aspec_topk_distill_fused_fwd_bwd", *call.head(flat),
+    pass_flags, ptr = call.check(flat, flags, waits), _lib.ptr
+    launch("topk_distill_fused", flat.device, pass_flags, "aspec_topk_distill_fused_fwd_bwd", *call.head(flat),
            call.renormalize, call.temperature, ptr(weights[0]), ptr(weights[1]), ptr(ce), kl.data_ptr(),
            accept.data_ptr(), ptr(amax), ptr(stats), ptr(workspace), grad.data_ptr(), row_stride(grad),
-           None if flags is None else flags.ptr)
+           None if pass_flags is None else pass_flags.ptr)
     if in_place and not logits.is_inference():
         torch.autograd.graph.increment_version(logits)  # a graph that kept the logits must not use them
     return (ce, kl, accept, logits if in_place else grad.view(logits.shape), amax), flags

@@ -383,6 +383,9 @@ int aspec_sampled_l1_bwd(const void* logits, const void* teacher, const int64_t*
  * aspec_token_logprobs_workspace_bytes (0 for most shapes; uninitialised; free once the call's
  * kernels are done).
  *
+ * aspec_token_logprobs_check sets the status word alone, in a kernel that takes a few microseconds: a
+ * host that must know before it goes on queues it ahead of the forward and waits for it.
+ *
  * aspec_token_logprobs_bwd writes the gradient of
  * sum (grad_logprobs logprobs + grad_entropy entropy + grad_top top_logprobs) (each may be NULL) in
  * the logits' dtype to grad_logits [rows][grad_stride], which is not the logits' buffer.
@@ -390,6 +393,8 @@ int aspec_sampled_l1_bwd(const void* logits, const void* teacher, const int64_t*
 int aspec_token_logprobs_stats_floats(void);
 int aspec_token_logprobs_workspace_bytes(int dtype, int64_t rows, int64_t vocab, int64_t top_k,
                                          size_t* bytes);
+int aspec_token_logprobs_check(const int64_t* token_ids, int64_t rows, int64_t vocab,
+                               int64_t ignore_index, int32_t* status_words, void* stream);
 int aspec_token_logprobs_fwd(const void* logits, int dtype, int64_t rows, int64_t vocab,
                              int64_t row_stride, const int64_t* token_ids, int64_t ignore_index,
                              float temperature, int64_t top_k, float* logprobs, float* entropy,
@@ -421,6 +426,8 @@ int aspec_token_logprobs_bwd(const void* logits, int dtype, int64_t rows, int64_
  * token twice in a row. workspace: of aspec_topk_distill_workspace_bytes (0 for most
  * shapes; uninitialised; free once the call's kernels are done).
  *
+ * aspec_topk_distill_check sets the status words alone, as aspec_token_logprobs_check does.
+ *
  * aspec_topk_distill_bwd writes the gradient of sum (grad_ce ce + grad_kl kl) (each may be NULL) in
  * the logits' dtype to grad_logits [rows][grad_stride], from the same teacher and the forward's
  * stats. aspec_topk_distill_fused_fwd_bwd is both in one call. It reads the logits
@@ -430,6 +437,11 @@ int aspec_token_logprobs_bwd(const void* logits, int dtype, int64_t rows, int64_
 int aspec_topk_distill_stats_floats(void);
 int aspec_topk_distill_workspace_bytes(int dtype, int64_t rows, int64_t vocab, size_t* bytes);
 int aspec_topk_distill_reads(int dtype, int64_t vocab);
+int aspec_topk_distill_check(int64_t rows, int64_t vocab, const int64_t* targets,
+                             int64_t ignore_index, const void* teacher_tokens, int token_dtype,
+                             const float* teacher_logprobs, int64_t kept,
+                             const int64_t* teacher_rows, int64_t num_teacher_rows,
+                             int32_t* status_words, void* stream);
 int aspec_topk_distill_fwd(const void* logits, int dtype, int64_t rows, int64_t vocab,
                            int64_t row_stride, const int64_t* targets, int64_t ignore_index,
                            const void* teacher_tokens, int token_dtype,

@@ -363,3 +363,21 @@ def test_extreme_temperatures(gpu, temperature):
         assert out.logprobs[0].item() == pytest.approx(-np.log(700), abs=2 * STEPS)
         assert out.entropy.tolist() == pytest.approx([np.log(700), np.log(699), np.log(700)], abs=16 * STEPS)
     assert out.logprobs[1].item() == -float("inf")
+
+
+@pytest.mark.parametrize("row", [0, 255, 256, 1099])
+@pytest.mark.parametrize("bad", [-1, 16000, 2**40])
+def test_a_bad_id_of_a_large_call_raises_before_it_returns(gpu, row, bad):
+    """Such a call checks its tokens in a kernel of their own, ahead of the logits' pass."""
+    from aspec_amd import _launch
+
+    x = torch.randn(1100, 16000, device=gpu, dtype=torch.bfloat16)
+    assert x.numel() * 2 >= _launch.CHECK_FIRST_BYTES
+    ids = torch.arange(1100, device=gpu)
+    ids[7] = -100
+    good = token_logprobs(x, ids)
+    assert torch.equal(good.logprobs, token_logprobs(x, ids, check_ids=False).logprobs)
+    ids[row] = bad
+    with pytest.raises(ValueError, match="token id out of range"):
+        token_logprobs(x, ids)
+    assert token_logprobs(x, ids, check_ids=False).logprobs[row].isnan()

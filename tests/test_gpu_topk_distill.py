@@ -456,3 +456,86 @@ def test_in_place_is_seen_by_autograd(gpu):
         assert out[3].data_ptr() == x.data_ptr() and torch.equal(x, logits.detach())
         assert torch.equal(topk_distill_from_logits(case.x, case.targets, case.tokens, case.logprobs)[1], out[1])
         assert token_logprobs(case.x, top_k=3).top_indices.shape == (4, 3)
+
+
+@pytest.mark.parametrize("token_dtype", [torch.int64, torch.int32])
+@pytest.mark.parametrize("kept", [1, 2, 63, 64, 65, 128])
+def test_the_check_ahead_of_the_pass_finds_what_the_pass_finds(gpu, monkeypatch, kept, token_dtype):
+    """The kernel that checks indices alone reports the words that the logits' pass reports, for one bad
+    row at either end and between, and none for tokens that only share their lower bits."""
+    from aspec_amd import _launch
+
+    rows, vocab, table = 7, 70000, 5
+    case = Case(gpu, rows, vocab, kept, torch.bfloat16, 71, table=table, fewer=False)
+    weights = {"ce_weights": torch.ones(rows, device=gpu), "kl_weights": torch.ones(rows, device=gpu)}
+
+    def verdicts(targets, tokens, where):
+        found = []
+        for limit in (0, 1 << 62):
+            monkeypatch.setattr(_launch, "CHECK_FIRST_BYTES", limit)
+            for entry, more in ((topk_distill_from_logits, {}), (topk_distill_fused_grad, weights)):
+                try:
+                    out = entry(case.x, targets, tokens, case.logprobs, teacher_rows=where, **more)
+                    found.append([v.isnan().any().item() for v in out])
+                except ValueError as e:
+                    found.append(str(e))
+        assert found[0] == found[2] and found[1] == found[3]
+        return found[0]
+
+    targets = torch.arange(rows, device=gpu)
+    where = torch.arange(rows, device=gpu) % table
+    tokens = torch.stack([torch.randperm(vocab, device=gpu)[:kept] for _ in range(table)])
+    if kept > 1:
+        tokens[0, :2] = torch.tensor([5, 5 + (1 << 15)], device=gpu)  # alike in the lower 15 bits
+        tokens[0, 2:] = torch.arange(100, 100 + kept - 2, device=gpu)
+    tokens = tokens.to(token_dtype)
+    assert verdicts(targets, tokens, where) == [False] * 3
+    unused = tokens.clone()
+    unused[:, kept // 2:] = -1
+    assert verdicts(targets, unused, where) == [False] * 3
+    for row in (0, 2, 4):
+        for slot in {0, kept // 2, kept - 1}:
+            for bad in (vocab, -2, 2**31 - 1):
+                changed = tokens.clone()
+                changed[row, slot] = bad
+                assert "teacher token out of range" in verdicts(targets, changed, where)
+            if slot:
+                changed = tokens.clone()
+                changed[row, slot] = changed[row, slot - 1]
+                assert "teacher token repeated" in verdicts(targets, changed, where)
+    if kept > 1:
+        changed = tokens.clone()
+        changed[3, kept - 1] = changed[3, 0]
+        assert "teacher token repeated" in verdicts(targets, changed, where)
+        # a table row that no row addresses may hold anything
+        assert verdicts(targets, changed, where.clamp(max=2)) == [False] * 3
+    for row in (0, 3, rows - 1):
+        for bad in (-1, vocab, 2**40):
+            changed = targets.clone()
+            changed[row] = bad
+            assert "cross-entropy target out of range" in verdicts(changed, tokens, where)
+        for bad in (-1, table, 2**40):
+            changed = where.clone()
+            changed[row] = bad
+            assert "teacher index out of range" in verdicts(targets, tokens, changed)
+
+
+def test_the_check_ahead_of_the_pass_is_taken_for_large_calls(gpu):
+    """Large enough that the check runs on its own: the error comes before the call returns, and the
+    results of good indices are the small calls'."""
+    rows, vocab = 1100, 16000
+    case = Case(gpu, rows, vocab, 3, torch.bfloat16, 72, fewer=False)
+    args = (case.targets, case.tokens, case.logprobs)
+    from aspec_amd import _launch
+
+    assert case.x.numel() * 2 >= _launch.CHECK_FIRST_BYTES
+    kl = topk_distill_from_logits(case.x, *args)[1]
+    small = topk_distill_from_logits(case.x[:40], case.targets[:40], case.tokens[:40], case.logprobs[:40])[1]
+    unchecked = topk_distill_from_logits(case.x, *args, check_indices=False)[1]
+    assert torch.equal(kl, unchecked)
+    torch.testing.assert_close(kl[:40], small, rtol=1e-4, atol=1e-5)
+    case.tokens[rows - 1, 2] = vocab
+    with pytest.raises(ValueError, match="teacher token out of range"):
+        topk_distill_from_logits(case.x, *args)
+    with pytest.raises(ValueError, match="teacher token out of range"):
+        topk_distill_fused_grad(case.x, *args, ce_weights=torch.ones(rows, device=gpu), kl_weights=torch.ones(rows, device=gpu))
