@@ -4,7 +4,7 @@ Drop-in replacements for the reference operators of aspec/models/ops (direct CP 
 the cuDNN FlexAttention surface with its DSpark interval masks, THD sparse metadata, tiled L1, the selective-head losses, the fused Q/K RMSNorm + RoPE, the DSpark
 head terms with the Markov bias and confidence head), the work-aware row packing policy
 (aspec/controller/packing.py), the packing collator (aspec/data/utils.py), the anchor layout (anchors.py), output-block compaction (output_blocks.py)
-and the DSpark targets (dspark.py), backed by hand-written HIP kernels in libaspec_amd.so,
+and the DSpark targets (dspark.py), token log-probabilities and distillation from a teacher's best tokens, backed by hand-written HIP kernels in libaspec_amd.so,
 reached through the C ABI of include/aspec_amd.h.
 """
 

@@ -6,10 +6,11 @@
 // registers; the kept tokens and the target, which have values of their own, are written behind the
 // dense ones by the thread that wrote those.
 //
-// 8192 x 32000 bf16, 64 kept tokens: forward 124-142 us (5.2-4.2 TB/s read, 521 MB), gradient 180 us
-// (1072 MB, 6.0 TB/s read and written). 1024 x 65536 fp32, 32 kept, forward alone: 43 us (6.2 TB/s). At
-// 16 rows a launch of 4.5-5 us each is the chain of one workgroup: the teacher's entries, their
-// logits, the row, the K-term sums in 64 bits.
+// 8192 x 32000 bf16, 64 kept tokens: forward 124-142 us behind the last gradient's writes (533 MB
+// read, VALU busy 0.8 with the second exponential of a temperature), gradient 180 us (1097 MB, 6.1 TB/s
+// read and written). 1024 x 65536 fp32, 32 kept, forward alone: 42 us (281 MB, 6.7 TB/s) and 5 us of
+// joining parts. At 16 rows each launch takes 4-5 us, the chain of one workgroup: the teacher's
+// entries, their logits, the row, the K-term sums in 64 bits.
 #include "topk_distill.h"
 
 namespace aspec {
