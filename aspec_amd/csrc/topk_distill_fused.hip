@@ -2,10 +2,10 @@
 // whole row in registers, takes its statistics and writes the row's gradient from there. Each logit
 // is read once and written once (the formulas are in topk_distill.h).
 //
-// HBM-bound up to 32768 16-bit logits to a row: 8192 x 32000 bf16, 64 kept tokens, 198 us for 1084 MB
-// (5.5 TB/s, a copy's rate; forward and gradient apart take 310). Longer rows take a workgroup of 1024
+// HBM-bound up to 32768 16-bit logits to a row: 8192 x 32000 bf16, 64 kept tokens, 195 us for 1084 MB
+// (5.6 TB/s, a copy's rate; forward and gradient apart take 310). Longer rows take a workgroup of 1024
 // threads with 80 of its 128 registers full of logits, one to a CU, so that nothing is read while a row
-// is reduced and written: 1536 x 151936 bf16 228 us (952 MB, 4.2 TB/s; forward and gradient apart read
+// is reduced and written: 1536 x 151936 bf16 223 us (952 MB, 4.3 TB/s; forward and gradient apart read
 // 480 MB more). Loading the next row ahead spilled 28-41 registers, whose reloads wait for those loads: 288.
 #include "topk_distill.h"
 

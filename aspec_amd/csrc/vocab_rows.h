@@ -262,26 +262,22 @@ struct Part {
     owner = in < 0 ? token : CH + token - (rc.lead + rc.chunks * CH);
     return NV * CH;
   }
-  // Sets the element at a place to -inf.
+  // Sets the element at a place to -inf: the masks of its word first, so that the branch for its chunk
+  // is one instruction a word (lanes whose chunks differ take the branches one after another; with the
+  // places compared in each branch 1536 x 151936 and 128 kept tokens took 228 us for 223).
   __device__ __forceinline__ void knock_out(int at) {
     if (at == NV * CH) edge = kNegInf;
+    const int i = at % CH, word = CH == 4 ? i : i / 2;
+    const uint32_t bits = CH == 4 ? ~0u : i % 2 ? 0xffff0000u : 0xffffu;
+    constexpr uint32_t none = CH == 4 ? E::kNegInfBits : E::kNegInfBits * 0x10001u;
+    uint32_t mask[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mask[j] = word == j ? bits : 0;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       if (v != at / CH) continue;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t old = word_of(w[v], j);
-        uint32_t now;
-        if constexpr (CH == 4) {
-          now = at % 4 == j ? E::kNegInfBits : old;
-        } else {
-          const int i = at % 8;
-          now = i == 2 * j       ? ((old & 0xffff0000u) | E::kNegInfBits)
-                : i == 2 * j + 1 ? ((old & 0xffffu) | (E::kNegInfBits << 16))
-                                 : old;
-        }
-        set_word(w[v], j, now);
-      }
+      for (int j = 0; j < 4; ++j) set_word(w[v], j, (word_of(w[v], j) & ~mask[j]) | (none & mask[j]));
     }
   }
   // Writes g(value) of every element to a row cut alike.
