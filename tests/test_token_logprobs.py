@@ -113,3 +113,19 @@ def test_refusals_of_the_c_entries():
     assert lib.aspec_token_logprobs_workspace_bytes(4, 4096, 32000, 64, ctypes.byref(size)) == 0 and size.value == 0
     assert lib.aspec_token_logprobs_workspace_bytes(4, 1, 151936, 20, ctypes.byref(size)) == 0 and size.value > 0
     fwd(rows=0)  # nothing to do
+
+
+def test_refusals_of_the_check_entry():
+    lib = _lib.load()
+    fake = ctypes.c_void_p(4096)  # never dereferenced: every call fails its checks, or has no rows
+
+    def check(ids=fake, rows=2, vocab=100, words=fake):
+        _lib.check(lib.aspec_token_logprobs_check(ids, rows, vocab, -100, words, None))
+
+    for error, match, bad in ((ValueError, "at least as far apart", {"rows": -1}),
+                              (ValueError, "at least as far apart", {"vocab": 0}),
+                              (NotImplementedError, "524288", {"vocab": 524289}),
+                              (ValueError, "null pointer", {"ids": None}), (ValueError, "null pointer", {"words": None})):
+        with pytest.raises(error, match=match):
+            check(**bad)
+    check(rows=0)

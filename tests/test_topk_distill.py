@@ -151,3 +151,26 @@ def test_refusals_of_the_c_entries():
     size = ctypes.c_size_t(1)
     assert lib.aspec_topk_distill_workspace_bytes(4, 8192, 32000, ctypes.byref(size)) == 0 and size.value == 0
     assert lib.aspec_topk_distill_workspace_bytes(4, 16, 32000, ctypes.byref(size)) == 0 and size.value > 0
+
+
+def test_refusals_of_the_check_entry():
+    lib = _lib.load()
+    fake = ctypes.c_void_p(4096)  # never dereferenced: every call fails its checks, or has no rows
+
+    def check(rows=2, vocab=100, tokens=fake, token_dtype=1, logprobs=fake, kept=5, teacher_rows=None,
+              num_teacher_rows=None, words=fake):
+        _lib.check(lib.aspec_topk_distill_check(
+            rows, vocab, fake, -100, tokens, token_dtype, logprobs, kept, teacher_rows,
+            rows if num_teacher_rows is None else num_teacher_rows, words, None))
+
+    for error, match, bad in (
+            (ValueError, "at least as far apart", {"rows": -1}), (ValueError, "at least as far apart", {"vocab": 0}),
+            (NotImplementedError, "524288", {"vocab": 524289}), (ValueError, "int64 or int32", {"token_dtype": 4}),
+            (ValueError, "a teacher token per row", {"kept": 0}), (NotImplementedError, "128", {"kept": 129}),
+            (ValueError, "a table of at least one", {"teacher_rows": fake, "num_teacher_rows": 0}),
+            (ValueError, "a table of at least one", {"num_teacher_rows": 3}),
+            (ValueError, "null pointer", {"tokens": None}), (ValueError, "null pointer", {"logprobs": None}),
+            (ValueError, "null pointer", {"words": None})):
+        with pytest.raises(error, match=match):
+            check(**bad)
+    check(rows=0)
