@@ -3,10 +3,12 @@
 // is read once and written once (the formulas are in topk_distill.h).
 //
 // HBM-bound up to 32768 16-bit logits to a row: 8192 x 32000 bf16, 64 kept tokens, 195 us for 1084 MB
-// (5.6 TB/s, a copy's rate; forward and gradient apart take 310). Longer rows take a workgroup of 1024
-// threads with 80 of its 128 registers full of logits, one to a CU, so that nothing is read while a row
-// is reduced and written: 1536 x 151936 bf16 223 us (952 MB, 4.3 TB/s; forward and gradient apart read
-// 480 MB more). Loading the next row ahead spilled 28-41 registers, whose reloads wait for those loads: 288.
+// (5.6 TB/s, a copy's rate; forward and gradient apart take 310). Longer rows fill 80 of a thread's 128
+// registers: up to 81920 logits 512 threads, two workgroups to a CU (8192 x 36000 244 us, 4.8 TB/s; 364
+// with 1024 threads of 10 chunks, one to a CU), beyond that 1024, one to a CU, so that nothing is read
+// while a row is reduced and written: 1536 x 151936 bf16 220 us (952 MB, 4.3 TB/s; forward and gradient
+// apart read 480 MB more). Loading the next row ahead spilled 28-41 registers, whose reloads wait for
+// those loads: 288.
 #include "topk_distill.h"
 
 namespace aspec {
@@ -15,7 +17,7 @@ namespace {
 using namespace distill;
 
 template <typename E, int T, int NV, bool TWO>
-__global__ __launch_bounds__(T, min_waves(T)) void topk_distill_fused_kernel(Args a) {
+__global__ __launch_bounds__(T, min_waves(NV)) void topk_distill_fused_kernel(Args a) {
   __shared__ Kept<T> kept;
   __shared__ float s_m[T / 64], s_s[T / 64], s_s1[T / 64];
   __shared__ uint64_t s_arg;
@@ -38,7 +40,7 @@ void launch_type(const Args& a, bool two, hipStream_t stream) {
   else if (a.part_chunks <= 256 * 4) launch<E, 256, 4>(a, two, stream);
   else if (a.part_chunks <= 512 * 4) launch<E, 512, 4>(a, two, stream);
   else if (a.part_chunks <= 512 * 8) launch<E, 512, 8>(a, two, stream);
-  else if (a.part_chunks <= 1024 * 10) launch<E, 1024, 10>(a, two, stream);
+  else if (a.part_chunks <= 512 * 20) launch<E, 512, 20>(a, two, stream);
   else launch<E, 1024, 20>(a, two, stream);
 }
 
