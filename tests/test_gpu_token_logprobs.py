@@ -381,3 +381,29 @@ def test_a_bad_id_of_a_large_call_raises_before_it_returns(gpu, row, bad):
     with pytest.raises(ValueError, match="token id out of range"):
         token_logprobs(x, ids)
     assert token_logprobs(x, ids, check_ids=False).logprobs[row].isnan()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("vocab,top_k", [(64, 64), (65, 7), (200, 60), (257, 128), (500, 64), (511, 1), (512, 128),
+                                         (1500, 64), (2047, 128), (2049, 128), (4099, 128)])
+def test_many_alternatives_of_few_tokens(gpu, vocab, top_k, dtype):
+    """Lists much longer than the number of alternatives: the same alternatives, in the same order, for
+    random, tied, masked and NaN rows."""
+    g = torch.Generator(device=gpu).manual_seed(vocab + top_k)
+    x = torch.randn(70, vocab, device=gpu, generator=g)
+    x[10:20] = x[10:20].mul(4).round().div(4)  # ties
+    x[20:24] = 1.5
+    x[24:30, torch.randperm(vocab, device=gpu, generator=g)[vocab // 3:]] = float("-inf")
+    x[30, ::7] = float("nan")
+    x[31] = float("nan")
+    x[32:40] = torch.arange(vocab, device=gpu).float() / 8
+    x[40:45] = -x[32:37]
+    x[45:50] = torch.finfo(dtype).min
+    x[45:50, vocab // 2] = 1.0
+    x = x.to(dtype)
+    got = token_logprobs(x, top_k=top_k)
+    order = O.top_order(x.float().cpu().numpy())[:, :top_k]
+    assert np.array_equal(got.top_indices.cpu().numpy(), order)
+    few = token_logprobs(x, top_k=1)
+    assert torch.equal(got.entropy.nan_to_num(7.0), few.entropy.nan_to_num(7.0))
+    assert torch.equal(got.top_logprobs[:, :1].nan_to_num(7.0), few.top_logprobs.nan_to_num(7.0))
