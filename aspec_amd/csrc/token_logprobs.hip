@@ -255,21 +255,17 @@ __global__ __launch_bounds__(T, 8) void token_logprobs_kernel(FwdArgs a) {
       }
       high = wave_allmax_u32(high);
       const uint32_t K = a.K, enough = K + K / 8 + 4;
-      const auto search = [&](auto held) {
-        constexpr int G = held.value;
+      const auto search = [&](const auto& group) {
+        constexpr int G = sizeof(group) / sizeof(uint32_t);
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-          if (w >= G) key[w % G] = max(key[w % G], key[w]);
-        }
-#pragma unroll
-        for (int w = 0; w < G; ++w) low = min(low, key[w]);
+        for (int w = 0; w < G; ++w) low = min(low, group[w]);
         low = wave_allmin(low);
         uint32_t top = high;
         while (low < top) {  // count(>= low) >= K throughout
           const uint32_t mid = low + (top - low) / 2 + ((top - low) & 1);
           uint32_t n = 0;
 #pragma unroll
-          for (int w = 0; w < G; ++w) n += __popcll(__ballot(key[w] >= mid));
+          for (int w = 0; w < G; ++w) n += __popcll(__ballot(group[w] >= mid));
           if (n >= K) {
             low = mid;
             if (n <= enough) break;
@@ -278,11 +274,25 @@ __global__ __launch_bounds__(T, 8) void token_logprobs_kernel(FwdArgs a) {
           }
         }
       };
-      if (K > T) low = 0;  // fewer maxima than tokens wanted: every token is listed
-      else if (W > 1 && K <= 16) search(std::integral_constant<int, 1>{});
-      else if (W > 2 && K <= 32) search(std::integral_constant<int, W < 2 ? W : 2>{});
-      else if (W > 4 && K <= 64) search(std::integral_constant<int, W < 4 ? W : 4>{});
-      else search(std::integral_constant<int, W>{});
+      const auto search_groups = [&](auto held) {
+        constexpr int G = held.value;
+        uint32_t group[G];
+#pragma unroll
+        for (int w = 0; w < W; ++w) group[w % G] = w < G ? key[w] : max(group[w % G], key[w]);
+        search(group);
+      };
+      if (W == 1 && K > 32) {
+        // the groups are half chunks, of which this wave holds the row's all: the 64 maxima alone leave the
+        // whole row to be listed (65536 x 2000 bf16 with 128 wanted: 309 us for 1082). With fewer half
+        // chunks than tokens wanted every token is listed too.
+        uint32_t group[2 * NV];
+#pragma unroll
+        for (int h = 0; h < 2 * NV; ++h) group[h] = order_key(p.largest_of_half(h));
+        search(group);
+      } else if (W > 1 && K <= 16) search_groups(std::integral_constant<int, 1>{});
+      else if (W > 2 && K <= 32) search_groups(std::integral_constant<int, W < 2 ? W : 2>{});
+      else if (W > 4 && K <= 64) search_groups(std::integral_constant<int, W < 4 ? W : 4>{});
+      else search_groups(std::integral_constant<int, W>{});
       if (lane == 0) {
         s_bound = low;
         s_high = high;
@@ -395,10 +405,10 @@ __global__ __launch_bounds__(T, 8) void token_logprobs_kernel(FwdArgs a) {
       __syncthreads();
     }
     int n = s_n;
-    if (n > 2 * a.K + 64) {
+    if (n > a.K + a.K / 2 + 32) {
       // ---- a list much longer than wanted (few groups for many tokens) is thinned out first, by the K-th
       // largest value in it or one a little below: the places take n^2 steps. 65536 x 500 bf16 with 64
-      // wanted, where every token is listed: 189 us for 1783.
+      // wanted, where every token was listed: 189 us for 1783.
       __syncthreads();
       if (wave == 0) {
         constexpr int H = kList / 64;

@@ -210,6 +210,14 @@ struct Part {
     }
   }
   __device__ __forceinline__ float largest() const { return fmaxf(largest_of<0, NV>(), edge); }
+  // The largest element of half of a chunk; a NaN is skipped, or is the result.
+  __device__ __forceinline__ float largest_of_half(int h) const {
+    constexpr int HALF = CH / 2;
+    float m = element<E>(w[h / 2], h % 2 * HALF);
+#pragma unroll
+    for (int i = 1; i < HALF; ++i) m = fmaxf(m, element<E>(w[h / 2], h % 2 * HALF + i));
+    return m;
+  }
   // One bit for each chunk whose largest element is not below a bound.
   template <int V = 0>
   __device__ __forceinline__ uint32_t chunks_reaching(float bound) const {
