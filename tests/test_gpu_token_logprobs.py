@@ -407,3 +407,19 @@ def test_many_alternatives_of_few_tokens(gpu, vocab, top_k, dtype):
     few = token_logprobs(x, top_k=1)
     assert torch.equal(got.entropy.nan_to_num(7.0), few.entropy.nan_to_num(7.0))
     assert torch.equal(got.top_logprobs[:, :1].nan_to_num(7.0), few.top_logprobs.nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("vocab", [700, 3001, 10240, 16777, 20000, 36001, 81919, 100003])
+def test_rows_between_the_shapes(gpu, vocab, dtype):
+    """Rows that leave places of a workgroup empty, from no wave's chunk to most of them."""
+    g = torch.Generator(device=gpu).manual_seed(vocab)
+    wide = (torch.randn(5, vocab + 5, device=gpu, generator=g) * 3).to(dtype)
+    for x in (wide[:, :vocab], wide[:, 3:3 + vocab]):
+        ids = torch.tensor([0, vocab - 1, vocab // 2, -100, 1], device=gpu)
+        got = token_logprobs(x, ids, top_k=100, temperature=0.8)
+        lp, entropy, top, order = O.forward(x.double().cpu().numpy(), ids.cpu().numpy(), 100, 0.8)
+        assert np.array_equal(got.top_indices.cpu().numpy(), order)
+        _close(got.logprobs, lp, STEPS + 4 * U * np.abs(lp), "logprobs")
+        _close(got.entropy, entropy, 2 * STEPS * (1 + entropy), "entropy")
+        _close(got.top_logprobs, top, STEPS + 4 * U * np.abs(top), "top_logprobs")

@@ -539,3 +539,17 @@ def test_the_check_ahead_of_the_pass_is_taken_for_large_calls(gpu):
         topk_distill_from_logits(case.x, *args)
     with pytest.raises(ValueError, match="teacher token out of range"):
         topk_distill_fused_grad(case.x, *args, ce_weights=torch.ones(rows, device=gpu), kl_weights=torch.ones(rows, device=gpu))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [3001, 10240, 16777, 20000, 33000, 36001, 65537, 81919, 100003, 123457])
+def test_rows_between_the_shapes(gpu, vocab, dtype):
+    """Rows that leave places of a workgroup empty, from no wave's chunk to most of them, with as many
+    kept tokens as fit, at temperature 1 and another."""
+    case = Case(gpu, 3, vocab, 128, dtype, vocab, temperature=0.8)
+    case.check()
+    Case(gpu, 3, vocab, 2, dtype, vocab + 1).check()
+    wide = torch.randn(3, vocab + 5, device=gpu, generator=torch.Generator(device=gpu).manual_seed(vocab)).to(dtype)
+    wide[:, 3:3 + vocab] = case.x
+    case.x = wide[:, 3:3 + vocab]  # rows that begin off a chunk's alignment
+    case.check()
